@@ -15,6 +15,7 @@ F32, F64, I32, BF16 = 0, 1, 2, 3
 _NP_DTYPE = {F32: np.float32, F64: np.float64, I32: np.int32}
 
 c_i64p = ctypes.POINTER(ctypes.c_int64)
+_I, _L, _D, _P, _S = ctypes.c_int, ctypes.c_int64, ctypes.c_double, ctypes.c_void_p, ctypes.c_size_t
 
 
 class DaliB200Error(RuntimeError):
@@ -76,6 +77,18 @@ class Library:
                                                ctypes.c_void_p]
         c.dalib200_scan.argtypes = [ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_int, ctypes.c_int, ctypes.c_int64,
                                     ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64, ctypes.c_void_p, ctypes.c_int64]
+        c.dalib200_layer_norm.argtypes = [_I, _P, _I, _I, _L, _L, _P, _L, _P, _P, _D, _P, _L]
+        c.dalib200_layer_norm_backward.argtypes = [_I, _P, _I, _I, _L, _L, _P, _L, _P, _L, _P, _D, _P, _L, _P, _P, _P, _S]
+        c.dalib200_layer_norm_backward_workspace.argtypes = [_I, _L, _L]
+        c.dalib200_token_logprobs.argtypes = [_I, _P, _I, _L, _L, _P, _L, _P, _P, _P, _P, _I, _P, _P]
+        c.dalib200_token_logprobs_backward.argtypes = [_I, _P, _I, _L, _L, _P, _L, _P, _P, _P, _P, _P, _P, _L]
+        c.dalib200_sum_squares.argtypes = [_I, _P, _I, _P, _P, _P, _P, _P, _S]
+        c.dalib200_global_norm.argtypes = [_I, _P, _I, _P, _P, _P, _I, _P, _P, _S]
+        c.dalib200_scale_to_norm.argtypes = [_I, _P, _I, _P, _P, _P, _P, _P, _D]
+        c.dalib200_clip_by_global_norm.argtypes = [_I, _P, _I, _P, _P, _P, _P, _D, _I, _P, _P, _S]
+        c.dalib200_global_norm_workspace.argtypes = [_I]
+        for name in ("dalib200_layer_norm_backward_workspace", "dalib200_global_norm_workspace"):
+            getattr(c, name).restype = ctypes.c_size_t
         c.dalib200_gemm_split_tf32_pair.argtypes = [ctypes.c_int, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p] + \
             [ctypes.c_int64] * 4 + [ctypes.c_void_p] * 4
         c.dalib200_gemm_error_flag.argtypes = [ctypes.c_int, ctypes.POINTER(ctypes.c_int)]
@@ -263,6 +276,86 @@ class Library:
         self.check(self.c.dalib200_scan(device, ctypes.c_void_p(stream or 0), dtype, op, int(bool(inclusive)), rows, cols,
                                         self._ptr(x), cols if in_row_stride is None else in_row_stride, self._ptr(out),
                                         (cols + (0 if inclusive else 1)) if out_row_stride is None else out_row_stride))
+
+    # -- operators of a token model (arguments that are None are left out, workspace: a CUDA tensor or None) ----------
+    @staticmethod
+    def _address(x):
+        return None if x is None else x.data_ptr() if hasattr(x, "data_ptr") else int(x)
+
+    @staticmethod
+    def _workspace(w):
+        return (None, 0) if w is None else (w.data_ptr(), w.numel() * w.element_size())
+
+    def layer_norm(self, dtype, param_dtype, rows, cols, x, gamma, beta, out, eps=1e-5, x_row_stride=None, out_row_stride=None,
+                   device=0, stream=None):
+        """out = (x - mean) / sqrt(var + eps) * gamma + beta along the rows of a [rows, cols] matrix."""
+        a = self._address
+        self.check(self.c.dalib200_layer_norm(device, stream, dtype, param_dtype, rows, cols, a(x),
+                                              cols if x_row_stride is None else x_row_stride, a(gamma), a(beta), eps, a(out),
+                                              cols if out_row_stride is None else out_row_stride))
+
+    def layer_norm_backward(self, dtype, param_dtype, rows, cols, dy, x, gamma, dx, dgamma, dbeta, eps=1e-5, dy_row_stride=None,
+                            x_row_stride=None, dx_row_stride=None, workspace=None, device=0, stream=None):
+        """The gradients of layer_norm; dx, dgamma and dbeta may be None."""
+        a = self._address
+        self.check(self.c.dalib200_layer_norm_backward(
+            device, stream, dtype, param_dtype, rows, cols, a(dy), cols if dy_row_stride is None else dy_row_stride, a(x),
+            cols if x_row_stride is None else x_row_stride, a(gamma), eps, a(dx), cols if dx_row_stride is None else dx_row_stride,
+            a(dgamma), a(dbeta), *self._workspace(workspace)))
+
+    def layer_norm_backward_workspace(self, dtype, rows, cols):
+        return self.c.dalib200_layer_norm_backward_workspace(dtype, rows, cols)
+
+    def token_logprobs(self, dtype, rows, vocab, logits, tokens, logprob, entropy, lse, top=0, top_logprobs=None, top_tokens=None,
+                       row_stride=None, device=0, stream=None):
+        """Log probability of the given token, entropy, log-sum-exp and the `top` most probable tokens of every row of logits."""
+        a = self._address
+        self.check(self.c.dalib200_token_logprobs(device, stream, dtype, rows, vocab, a(logits), vocab if row_stride is None else row_stride,
+                                                  a(tokens), a(logprob), a(entropy), a(lse), top, a(top_logprobs), a(top_tokens)))
+
+    def token_logprobs_backward(self, dtype, rows, vocab, logits, tokens, lse, entropy, dlogprob, dentropy, dlogits, row_stride=None,
+                                dlogits_row_stride=None, device=0, stream=None):
+        """The gradient of token_logprobs' logprob and entropy with respect to the logits."""
+        a = self._address
+        self.check(self.c.dalib200_token_logprobs_backward(
+            device, stream, dtype, rows, vocab, a(logits), vocab if row_stride is None else row_stride, a(tokens), a(lse), a(entropy),
+            a(dlogprob), a(dentropy), a(dlogits), vocab if dlogits_row_stride is None else dlogits_row_stride))
+
+    def _tensor_list(self, dtypes, numel, tensors):
+        n = len(tensors)
+        if len(dtypes) != n or len(numel) != n:
+            raise ValueError("dtypes, numel and tensors must have one entry per tensor")
+        a = self._address
+        return n, (_I * n)(*dtypes), (_L * n)(*numel), (_P * n)(*[a(x) for x in tensors])
+
+    def sum_squares(self, dtypes, numel, tensors, out, workspace=None, device=0, stream=None):
+        """*out (fp64) = sum of the squares of all elements of a list of contiguous tensors."""
+        self.check(self.c.dalib200_sum_squares(device, stream, *self._tensor_list(dtypes, numel, tensors), self._address(out),
+                                               *self._workspace(workspace)))
+
+    def global_norm(self, dtypes, numel, tensors, norm, norm_dtype=F32, workspace=None, device=0, stream=None):
+        """*norm = the norm of a list of contiguous tensors taken as one vector."""
+        self.check(self.c.dalib200_global_norm(device, stream, *self._tensor_list(dtypes, numel, tensors), norm_dtype,
+                                               self._address(norm), *self._workspace(workspace)))
+
+    def _outs(self, n, outs):
+        if len(outs) != n:
+            raise ValueError("outs must have one entry per tensor")
+        return (_P * n)(*[self._address(x) for x in outs])
+
+    def scale_to_norm(self, dtypes, numel, tensors, outs, sum_squares, max_norm, device=0, stream=None):
+        """outs[i] = tensors[i] * min(1, max_norm / sqrt(*sum_squares))."""
+        args = self._tensor_list(dtypes, numel, tensors)
+        self.check(self.c.dalib200_scale_to_norm(device, stream, *args, self._outs(args[0], outs), self._address(sum_squares), max_norm))
+
+    def clip_by_global_norm(self, dtypes, numel, tensors, outs, max_norm, norm, norm_dtype=F32, workspace=None, device=0, stream=None):
+        """outs[i] = tensors[i] * min(1, max_norm / n), n the norm of all of them, which is left in *norm."""
+        args = self._tensor_list(dtypes, numel, tensors)
+        self.check(self.c.dalib200_clip_by_global_norm(device, stream, *args, self._outs(args[0], outs), max_norm, norm_dtype,
+                                                       self._address(norm), *self._workspace(workspace)))
+
+    def global_norm_workspace(self, n_tensors):
+        return self.c.dalib200_global_norm_workspace(n_tensors)
 
     def gemm_split_tf32_pair(self, x0, x1, rows, cols, ld0, ld1, hi0, lo0, hi1, lo1, device=0, stream=None):
         self.check(self.c.dalib200_gemm_split_tf32_pair(device, ctypes.c_void_p(stream or 0), self._ptr(x0), self._ptr(x1), rows,

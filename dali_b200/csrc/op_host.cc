@@ -1,0 +1,57 @@
+// Workspaces of the hand-written operators (op_host.h).
+#include "op_host.h"
+
+#include <algorithm>
+#include <map>
+#include <utility>
+
+namespace dalib {
+
+std::mutex& launch_mutex() {
+    static std::mutex* m = new std::mutex();
+    return *m;
+}
+
+namespace {
+struct Space { void* data = nullptr; size_t bytes = 0; };
+// apart from the exchange space of generated kernels: those are queued without the launch mutex
+std::map<std::pair<int, void*>, Space>& spaces() {
+    static auto* m = new std::map<std::pair<int, void*>, Space>();
+    return *m;
+}
+}  // namespace
+
+int workspace_for(int device, void* stream, size_t need, void* given, size_t given_bytes, void** out) {
+    if (given) {
+        if (given_bytes < need) return refuse("workspace of " + std::to_string(given_bytes) + " bytes, " + std::to_string(need) + " are needed");
+        if ((uintptr_t)given % 16) return refuse("workspace is not 16-byte aligned");
+        *out = given;
+        return DALIB200_OK;
+    }
+    if ((cudaStream_t)stream == cudaStreamPerThread) return refuse("a call on the per-thread default stream needs a workspace of its own");
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    const cudaError_t asked = cudaStreamIsCapturing((cudaStream_t)stream, &st);
+    if (asked != cudaSuccess || st != cudaStreamCaptureStatusNone) {
+        cudaGetLastError();
+        return refuse("a call that is captured into a graph needs a workspace of its own");
+    }
+    Space& s = spaces()[std::make_pair(device, stream)];
+    if (s.bytes < need) {
+        // (kernels in flight may still use the old block: cudaFree waits for the device)
+        const size_t bytes = std::max<size_t>(need, 4u << 20);
+        void* fresh = nullptr;
+        const cudaError_t e = cudaMalloc(&fresh, bytes);
+        if (e != cudaSuccess) {
+            cudaGetLastError();
+            set_error(std::string("workspace: cudaMalloc: ") + cudaGetErrorString(e));
+            return DALIB200_ERR_CUDA;
+        }
+        if (s.data) cudaFree(s.data);
+        s.data = fresh;
+        s.bytes = bytes;
+    }
+    *out = s.data;
+    return DALIB200_OK;
+}
+
+}  // namespace dalib

@@ -253,6 +253,80 @@ int dalib200_scan(int device, void* stream, int dtype, int op, int inclusive,
                   int64_t rows, int64_t cols, const void* in, int64_t in_row_stride,
                   void* out, int64_t out_row_stride);
 
+/* ---- operators of a token model -----------------------------------------------
+ * No counterpart in the reference, whose layers stop at softmax and its cross entropy: layer normalisation, log
+ * probabilities of tokens and gradient clipping, each with what a training step needs of it.
+ *
+ * Matrices are row-major with a unit inner stride and a row stride in elements; rows may start at any element.  dtype is
+ * f32, f64 or bf16 (values widen to fp32, results round to nearest even); statistics, sums and log probabilities are held
+ * in fp32, in fp64 for f64.  Everything is asynchronous on `stream`.  An output may be the matrix it is computed from
+ * (`out == x`, `dx == dy` or `dx == x`, `dlogits == logits`, each with the same row stride); any other overlap of an output
+ * with another argument is refused.  NULL stands for an argument that is marked optional.
+ *
+ * Workspaces: operators that take one pass partial results from one launch to the next through it.  NULL: the library's own
+ * space of (device, stream), which the next call on that stream reuses.  A call that is captured into a graph, or that runs
+ * on the per-thread default stream, has to bring its own (16-byte aligned, of at least the size that the operator's
+ * _workspace function gives) and may share it only with calls that cannot run at the same time. */
+
+/* out = (x - mean) / sqrt(var + eps) * gamma + beta along the rows of the [rows, cols] matrix x, mean and (biased) variance
+ * taken per row.  gamma, beta: `cols` values of param_dtype, each optional (1 and 0).  param_dtype is dtype, or f32 beside
+ * bf16 rows.  eps >= 0.  Squared deviations are held in fp32: deviations beyond 1e19 overflow in f32 and bf16 rows. */
+int dalib200_layer_norm(int device, void* stream, int dtype, int param_dtype, int64_t rows, int64_t cols,
+                        const void* x, int64_t x_row_stride, const void* gamma, const void* beta, double eps,
+                        void* out, int64_t out_row_stride);
+/* The gradients of dalib200_layer_norm for the gradient dy of its result: dx [rows, cols], and dgamma, dbeta (`cols` values
+ * of param_dtype, overwritten), each of the three optional.  The rows' statistics are computed again from x.  The sums over the rows
+ * are taken in a fixed order: the same call gives the same bits. */
+int dalib200_layer_norm_backward(int device, void* stream, int dtype, int param_dtype, int64_t rows, int64_t cols,
+                                 const void* dy, int64_t dy_row_stride, const void* x, int64_t x_row_stride,
+                                 const void* gamma, double eps, void* dx, int64_t dx_row_stride, void* dgamma, void* dbeta,
+                                 void* workspace, size_t workspace_bytes);
+size_t dalib200_layer_norm_backward_workspace(int dtype, int64_t rows, int64_t cols);
+
+/* Per row of the [rows, vocab] matrix of logits z: lse = log sum exp z; logprob = z[token] - lse; entropy = - sum p log p of
+ * p = exp(z - lse); and the `top` most probable tokens with their log probabilities, [rows, top], most probable first, among
+ * equal ones the lowest index first.  Each result is optional (top = 0: no alternatives); f32 values, f64 for f64 logits.
+ *   tokens      int32; a negative one marks a row without a token: its logprob is 0.  A token >= vocab gives NaN.
+ *   logits      -infinity marks a token that cannot be drawn (its logprob is -infinity, it takes no part in the sums).  A row of
+ *               nothing else has lse = logprob = -infinity, entropy 0 and alternatives 0, 1, 2, ... of -infinity.  NaN
+ *               or +infinity anywhere in a row makes its results NaN; NaN entries rank behind all others among the alternatives.
+ *   top         0 .. DALIB200_MAX_TOP, at most vocab
+ * vocab < 2^31. */
+#define DALIB200_MAX_TOP 32
+int dalib200_token_logprobs(int device, void* stream, int dtype, int64_t rows, int64_t vocab,
+                            const void* logits, int64_t row_stride, const int32_t* tokens,
+                            void* logprob, void* entropy, void* lse, int top, void* top_logprobs, int32_t* top_tokens);
+/* The gradient of logprob and entropy with respect to the logits, for the gradients dlogprob and dentropy that arrive (`rows`
+ * values each, either optional) and the lse and entropy that the forward pass gave:
+ *   dlogits[j] = dlogprob ([j == token] - p_j) - dentropy p_j (log p_j + entropy)
+ * A row without a token (negative) takes dlogprob as 0; a token >= vocab makes its row NaN.  Rows whose gradients are both
+ * 0, and rows of nothing but -infinity, get 0 whatever their logits hold.  entropy is needed with dentropy only, tokens
+ * with dlogprob only. */
+int dalib200_token_logprobs_backward(int device, void* stream, int dtype, int64_t rows, int64_t vocab,
+                                     const void* logits, int64_t row_stride, const int32_t* tokens,
+                                     const void* lse, const void* entropy, const void* dlogprob, const void* dentropy,
+                                     void* dlogits, int64_t dlogits_row_stride);
+
+/* Lists of tensors (host arrays of n_tensors dtypes, element counts and device pointers; contiguous; f32, f64 and bf16 may be
+ * mixed; empty ones are skipped), read when the call is made:
+ *   sum_squares          *sum = sum of the squares of all elements, fp64
+ *   global_norm          *norm = its square root (norm_dtype f32 or f64)
+ *   scale_to_norm        outs[i] = tensors[i] * min(1, max_norm / n), n = sqrt(*sum_squares): for lists that are spread over
+ *                        ranks, whose sums of squares are added (dalib200_allreduce) in between
+ *   clip_by_global_norm  all of it: *norm is the norm before scaling
+ * outs[i] may be tensors[i]; nothing that is written may overlap anything else of the list.  max_norm > 0.  A norm that is
+ * not finite scales nothing: outs[i] = tensors[i], and *norm says so.  Sums are taken in fp64 in a fixed order. */
+int dalib200_sum_squares(int device, void* stream, int n_tensors, const int* dtypes, const int64_t* numel,
+                         const void* const* tensors, double* sum, void* workspace, size_t workspace_bytes);
+int dalib200_global_norm(int device, void* stream, int n_tensors, const int* dtypes, const int64_t* numel,
+                         const void* const* tensors, int norm_dtype, void* norm, void* workspace, size_t workspace_bytes);
+int dalib200_scale_to_norm(int device, void* stream, int n_tensors, const int* dtypes, const int64_t* numel,
+                           const void* const* tensors, void* const* outs, const double* sum_squares, double max_norm);
+int dalib200_clip_by_global_norm(int device, void* stream, int n_tensors, const int* dtypes, const int64_t* numel,
+                                 const void* const* tensors, void* const* outs, double max_norm, int norm_dtype, void* norm,
+                                 void* workspace, size_t workspace_bytes);
+size_t dalib200_global_norm_workspace(int n_tensors);
+
 /* ---- allocation-free entry point ----------------------------------------------
  * No counterpart in the reference (it allocates freely through memory::bank).
  *
