@@ -320,6 +320,10 @@ def _wrap(x):
     return Array(np.asarray(x))
 
 
+def _opt(a):
+    return None if a is None else a._h
+
+
 class _Op:
     """namespace op:: of the reference (dali/array/op.h)."""
 
@@ -361,6 +365,43 @@ class _Op:
 
     def softmax(self, logits, axis=-1):
         return Array._new(_c().c.dali_op_softmax, logits._h, int(axis))
+
+    # ---- operators of a token model (gamma, beta, tokens ... may be None where dali/array/op.h lets them be left out)
+    @staticmethod
+    def _several(fn, n, *args):
+        handles = [_H() for _ in range(n)]
+        _check(fn(*args, *[ctypes.byref(h) for h in handles]))
+        return tuple(Array(_handle=h) for h in handles)
+
+    def layer_norm(self, x, gamma=None, beta=None, eps=1e-5):
+        return Array._new(_c().c.dali_op_layer_norm, _opt(x), _opt(gamma), _opt(beta), ctypes.c_double(eps))
+
+    def layer_norm_backward(self, dy, x, gamma=None, eps=1e-5):
+        """(dx, dgamma, dbeta)"""
+        return self._several(_c().c.dali_op_layer_norm_backward, 3, _opt(dy), _opt(x), _opt(gamma), ctypes.c_double(eps))
+
+    def token_logprobs(self, logits, tokens=None, top=0):
+        """(logprob, entropy, lse, top_logprobs, top_tokens); logprob is None without tokens, the last two without top."""
+        tokens = None if tokens is None else _wrap(tokens)
+        want = [tokens is not None, True, True, top > 0, top > 0]
+        handles = [_H() if w else None for w in want]
+        _check(_c().c.dali_op_token_logprobs(_opt(logits), _opt(tokens), int(top), *[None if h is None else ctypes.byref(h) for h in handles]))
+        return tuple(None if h is None else Array(_handle=h) for h in handles)
+
+    def token_logprobs_backward(self, logits, tokens, lse, entropy, dlogprob, dentropy=None):
+        keep = [None if a is None else _wrap(a) for a in (logits, tokens, lse, entropy, dlogprob, dentropy)]
+        return Array._new(_c().c.dali_op_token_logprobs_backward, *[_opt(a) for a in keep])
+
+    def global_norm(self, arrays):
+        return Array._new(_c().c.dali_op_global_norm, (_H * max(len(arrays), 1))(*[a._h for a in arrays]), len(arrays))
+
+    def clip_by_global_norm(self, arrays, max_norm):
+        """([clipped arrays], norm before clipping)"""
+        n = len(arrays)
+        clipped, norm = (_H * max(n, 1))(), _H()
+        _check(_c().c.dali_op_clip_by_global_norm((_H * max(n, 1))(*[a._h for a in arrays]), n, ctypes.c_double(max_norm), clipped,
+                                                  ctypes.byref(norm)))
+        return [Array(_handle=_H(clipped[i])) for i in range(n)], Array(_handle=norm)
 
     def dot(self, a, b):
         return Array._new(_c().c.dali_op_dot, a._h, b._h)

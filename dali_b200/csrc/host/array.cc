@@ -637,6 +637,7 @@ Array Array::reshape(const std::vector<int>& new_shape_) const {
 Array Array::ravel() const { return reshape({-1}); }
 
 Array Array::ascontiguousarray() const {
+    if (!is_stateless() && expression()->kind_ == N_KERNEL) eval(false);      // contiguous as its kernel leaves it, and not computed again
     if (is_buffer() && as<BufferView>(*this)->contiguous()) return *this;
     Array out(shape(), dtype(), preferred_device());
     out.expression()->shard_ = shard();

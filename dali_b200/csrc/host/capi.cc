@@ -47,6 +47,8 @@ size_t copy_out(const std::string& s, char* buffer, size_t capacity) {
     return s.size();
 }
 
+Array optional(dali_array_t h) { return h ? h->a : Array(); }
+
 dali_array_t wrap(const Array& a) {
     dali_array_s* h = new dali_array_s();
     h->a = a;
@@ -289,6 +291,56 @@ int dali_random_set_seed(int seed) {
 }
 int dali_op_softmax(dali_array_t logits, int axis, dali_array_t* out) {
     return guard([&]() { *out = wrap(op::softmax(logits->a, axis)); });
+}
+int dali_op_layer_norm(dali_array_t x, dali_array_t gamma, dali_array_t beta, double eps, dali_array_t* out) {
+    return guard([&]() { *out = wrap(op::layer_norm(x->a, optional(gamma), optional(beta), eps)); });
+}
+int dali_op_layer_norm_backward(dali_array_t dy, dali_array_t x, dali_array_t gamma, double eps, dali_array_t* dx, dali_array_t* dgamma,
+                                dali_array_t* dbeta) {
+    return guard([&]() {
+        Array a, b, c;
+        std::tie(a, b, c) = op::layer_norm_backward(dy->a, x->a, optional(gamma), eps);
+        if (dx) *dx = wrap(a);
+        if (dgamma) *dgamma = wrap(b);
+        if (dbeta) *dbeta = wrap(c);
+    });
+}
+int dali_op_token_logprobs(dali_array_t logits, dali_array_t tokens, int top, dali_array_t* logprob, dali_array_t* entropy,
+                           dali_array_t* lse, dali_array_t* top_logprobs, dali_array_t* top_tokens) {
+    return guard([&]() {
+        DALI_ASSERT(!logprob || tokens, "token_logprobs: logprob needs tokens");
+        DALI_ASSERT((!top_logprobs && !top_tokens) || top > 0, "token_logprobs: no alternatives without top > 0");
+        op::TokenLogprobs r = op::token_logprobs(logits->a, optional(tokens), top);
+        if (logprob) *logprob = wrap(r.logprob);
+        if (entropy) *entropy = wrap(r.entropy);
+        if (lse) *lse = wrap(r.lse);
+        if (top_logprobs) *top_logprobs = wrap(r.top_logprobs);
+        if (top_tokens) *top_tokens = wrap(r.top_tokens);
+    });
+}
+int dali_op_token_logprobs_backward(dali_array_t logits, dali_array_t tokens, dali_array_t lse, dali_array_t entropy,
+                                    dali_array_t dlogprob, dali_array_t dentropy, dali_array_t* out) {
+    return guard([&]() {
+        *out = wrap(op::token_logprobs_backward(logits->a, optional(tokens), lse->a, optional(entropy), optional(dlogprob),
+                                                optional(dentropy)));
+    });
+}
+int dali_op_global_norm(const dali_array_t* arrays, int n, dali_array_t* out) {
+    return guard([&]() {
+        std::vector<Array> v;
+        for (int i = 0; i < n; ++i) v.push_back(arrays[i]->a);
+        *out = wrap(op::global_norm(v));
+    });
+}
+int dali_op_clip_by_global_norm(const dali_array_t* arrays, int n, double max_norm, dali_array_t* clipped, dali_array_t* norm) {
+    return guard([&]() {
+        std::vector<Array> v, c;
+        Array total;
+        for (int i = 0; i < n; ++i) v.push_back(arrays[i]->a);
+        std::tie(c, total) = op::clip_by_global_norm(v, max_norm);
+        for (int i = 0; i < n; ++i) clipped[i] = wrap(c[i]);
+        if (norm) *norm = wrap(total);
+    });
 }
 int dali_op_dot(dali_array_t a, dali_array_t b, dali_array_t* out) {
     return guard([&]() { *out = wrap(op::dot(a->a, b->a)); });

@@ -126,6 +126,15 @@ Array canonical(const Array& array) {
     }
     expression_ptr e = array.expression();
     if (e->kind_ == N_BUFFER || e->kind_ == N_ASSIGN) return array;
+    if (e->kind_ == N_KERNEL) {
+        // its kernel writes a fresh buffer of its own
+        KernelResult* k = static_cast<KernelResult*>(e.get());
+        std::string name;
+        if (Scope::has_observers()) name = array.full_expression_name();
+        DALI_SCOPE(name);
+        array.set_expression(k->call_->take(k->index_).expression());
+        return array;
+    }
     // wrap the value in an assignment to a fresh buffer (optimization.cpp:29-67 does this for every node that is not
     // assignable; here only the root needs it -- what cannot share the root's kernel is given its own assignment
     // during lowering).  The buffer is the same part of a logical array as the value.

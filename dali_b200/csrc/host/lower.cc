@@ -400,6 +400,7 @@ struct Lowerer {
                 break;
             }
             case N_SCAN:
+            case N_KERNEL:
                 // never fused with what consumes it (dali/array/op/scan.cpp:37-39: chainable() is false)
                 id = visit(materialize(a), m);
                 break;
@@ -1258,6 +1259,13 @@ void run_assignment(const Array& dest_in, OPERATOR_T op, const Array& value_in) 
     // ---- a running reduction at the root has its own kernel
     if (value.expression()->kind_ == N_SCAN && dest.is_buffer()) {
         run_scan(dest, op, static_cast<Scan*>(value.expression().get()));
+        return;
+    }
+
+    // ---- a result of an operator with a kernel of its own
+    if (value.expression()->kind_ == N_KERNEL) {
+        value.eval(false);      // (whoever shares this handle finds it evaluated)
+        run_assignment(dest, op, value);
         return;
     }
 

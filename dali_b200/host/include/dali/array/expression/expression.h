@@ -21,7 +21,7 @@
 
 #include "dali/array/array.h"
 
-enum NodeKind { N_BUFFER, N_SCALAR, N_ELEMENTWISE, N_REDUCE, N_VIEW, N_GATHER, N_GATHER_ROWS, N_MATMUL, N_ASSIGN, N_IOTA, N_SCAN };
+enum NodeKind { N_BUFFER, N_SCALAR, N_ELEMENTWISE, N_REDUCE, N_VIEW, N_GATHER, N_GATHER_ROWS, N_MATMUL, N_ASSIGN, N_IOTA, N_SCAN, N_KERNEL };
 
 class Expression {
   public:
@@ -86,6 +86,34 @@ struct Scan : public Expression {
     bool inclusive_;
     Scan(const Array& a, const std::string& reducer, bool inclusive);
     std::string name() const override { return std::string(inclusive_ ? "inclusive_" : "exclusive_") + "scan_" + reducer_; }
+};
+
+// An operator with a hand-written kernel of its own and one or more results (layer_norm_backward's three gradients): the
+// first result that is asked for runs it, the others find theirs computed.  Like a Scan it is never fused with what
+// consumes it.  Results nobody holds a node of any more are not computed (of whole arrays; of shards they are, so that all
+// ranks take the same collective steps).
+struct KernelResult;
+struct KernelCall {
+    struct Result { std::string name; std::vector<int> shape; DType dtype; Shard shard; };
+    std::vector<Array> inputs_;                              // stateless: an optional input that is left out
+    std::vector<Result> results_;
+    virtual ~KernelCall() {}
+    virtual std::string name() const = 0;
+    // inputs as evaluated buffers; outputs[i] is stateless where the result is not wanted
+    virtual void run(const memory::Device& device, const std::vector<Array>& inputs, const std::vector<Array>& outputs) = 0;
+    // the lazy Arrays of `call`'s results, one for each
+    static std::vector<Array> lazy_results(const std::shared_ptr<KernelCall>& call);
+    // the evaluated result: computed now, or left by the run that another result asked for (each is handed out once)
+    Array take(int index);
+  private:
+    std::vector<Array> computed_;
+    std::vector<std::weak_ptr<KernelResult>> nodes_;
+};
+struct KernelResult : public Expression {
+    std::shared_ptr<KernelCall> call_;
+    int index_;
+    KernelResult(const std::shared_ptr<KernelCall>& call, int index);
+    std::string name() const override { return call_->name() + "." + call_->results_[index_].name; }
 };
 
 // functor(arg0[, arg1]); rank-0 arguments broadcast implicitly.

@@ -105,6 +105,24 @@ Array gather_from_rows(const Array& source, const Array& indices);
 Array softmax(const Array& logits, int axis = -1);
 Array softmax_temperature(const Array& logits, const Array& temperature, int axis = -1);
 
+// ---- operators of a token model (op/token_model.h; not in the reference).  Lazy, each with a kernel of its own.  Rows run
+// along the last axis.  Unlike other computations they keep a bf16 type of their rows: a result with the shape of a
+// bf16 argument is bf16 (computed in fp32, rounded once when it is stored).
+// (x - mean) / sqrt(var + eps) * gamma + beta; gamma / beta: vectors of the last axis' length, stateless = left out
+Array layer_norm(const Array& x, const Array& gamma, const Array& beta, double eps = 1e-5);
+// its gradients for the gradient dy of its result: (dx, dgamma, dbeta)
+std::tuple<Array, Array, Array> layer_norm_backward(const Array& dy, const Array& x, const Array& gamma, double eps = 1e-5);
+// per row of logits [..., vocab]: log probability of the given token (int32, [...]; negative = none, 0 is returned;
+// stateless = not asked for), entropy, log-sum-exp, and the `top` most probable tokens, [..., top] (top = 0: stateless)
+struct TokenLogprobs { Array logprob, entropy, lse, top_logprobs, top_tokens; };
+TokenLogprobs token_logprobs(const Array& logits, const Array& tokens, int top = 0);
+// gradient of logprob and entropy with respect to the logits; dlogprob (with tokens) or dentropy (with entropy) may be stateless
+Array token_logprobs_backward(const Array& logits, const Array& tokens, const Array& lse, const Array& entropy, const Array& dlogprob,
+                              const Array& dentropy);
+// norm of all arrays taken as one vector (float; double if one of them is), and the arrays scaled by min(1, max_norm / norm)
+Array global_norm(const std::vector<Array>& arrays);
+std::tuple<std::vector<Array>, Array> clip_by_global_norm(const std::vector<Array>& arrays, double max_norm);
+
 // ---- dot
 Array matmul(Array a, Array b);
 Array matrix_vector_dot(const Array& a, const Array& b);

@@ -97,6 +97,18 @@ int dali_op_arange(dali_array_t start, dali_array_t stop, dali_array_t step, dal
 int dali_op_random(const char* kind, dali_array_t a, dali_array_t b, const int64_t* shape, int ndim, dali_array_t* out);
 int dali_random_set_seed(int seed);
 int dali_op_softmax(dali_array_t logits, int axis, dali_array_t* out);
+/* operators of a token model (not in the reference; the C++ functions of the same names in dali/array/op.h, the entry points
+ * behind them in dali_b200.h).  NULL handles: gamma, beta, tokens, and one of the pairs tokens + dlogprob and entropy + dentropy may
+ * be left out; NULL results are not wanted. */
+int dali_op_layer_norm(dali_array_t x, dali_array_t gamma, dali_array_t beta, double eps, dali_array_t* out);
+int dali_op_layer_norm_backward(dali_array_t dy, dali_array_t x, dali_array_t gamma, double eps, dali_array_t* dx, dali_array_t* dgamma,
+                                dali_array_t* dbeta);
+int dali_op_token_logprobs(dali_array_t logits, dali_array_t tokens, int top, dali_array_t* logprob, dali_array_t* entropy,
+                           dali_array_t* lse, dali_array_t* top_logprobs, dali_array_t* top_tokens);
+int dali_op_token_logprobs_backward(dali_array_t logits, dali_array_t tokens, dali_array_t lse, dali_array_t entropy,
+                                    dali_array_t dlogprob, dali_array_t dentropy, dali_array_t* out);
+int dali_op_global_norm(const dali_array_t* arrays, int n, dali_array_t* out);
+int dali_op_clip_by_global_norm(const dali_array_t* arrays, int n, double max_norm, dali_array_t* clipped /* n */, dali_array_t* norm);
 int dali_op_dot(dali_array_t a, dali_array_t b, dali_array_t* out);
 
 /* ---- assignment (array.h:201-205, 233-241): op 0 '=', 1 '+=', 2 '-=', 3 '*=', 4 '/=', 5 '<<=' */
