@@ -11,6 +11,7 @@
 // An entry of -infinity is one that cannot be drawn (p = 0, 0 log 0 = 0); a row of nothing else has lse = -infinity,
 // logprob = -infinity and H = 0.  The alternatives are ordered by value and, among equal values, by index; NaN ranks last.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "op_device.cuh"
@@ -114,7 +115,7 @@ __device__ __forceinline__ void finish_row(const Running<A>& all, long long row,
 template <typename A>
 __device__ __forceinline__ A log_p(A z, A lse) { return lse == -infinity_of(A()) ? lse : z - lse; }
 
-// ---------------------------------------------------------------------------------------------- simplest form
+// ---------------------------------------------------------------------------------------------- f64 rows
 // A CTA per row, one entry a thread and step; the alternatives one after another, each by another walk over the row.
 template <typename T>
 __global__ void __launch_bounds__(kThreads) logprobs_rows_kernel(const T* __restrict__ logits, long long ld, long long rows, int vocab,
@@ -180,6 +181,390 @@ __global__ void __launch_bounds__(kThreads) logprobs_rows_kernel(const T* __rest
     }
 }
 
+// ---------------------------------------------------------------------------------------------- f32 and bf16 rows
+// A cluster of S CTAs shares a row, each a contiguous slice of its 16-byte packets; a thread takes every kThreads-th packet of
+// its CTA's slice, kBatch of them at a time, and keeps (m, s, u) in units of log 2: t = (z - m) log2 e, s = sum 2^t,
+// u = sum t 2^t.  (z - m is formed before it is scaled: a row of the type's lowest value is uniform, not -infinity.)
+//
+// The alternatives cost no work in that pass.  The entries of one thread are a GROUP; a thread remembers in which batch its
+// maximum was raised last.  At least `top` entries are >= the top-th largest group maximum tau (by value, then index: a total order),
+// and every entry >= tau lies in one of those `top` groups: only they are read again (from L2, 1 / 256 of a CTA's slice each), and
+// what is >= tau in them, hardly more than `top` entries, is sorted.  Lists of 32 keys, one a lane, are sorted and merged
+// bitonically.
+constexpr int kBatch = 4;
+constexpr int kWarps = kThreads / 32;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kFloor = -290.0f;              // 2^t is 0 in fp32 below; t does not fall lower, so that 0 * t stays 0 for t = -infinity
+
+__device__ __forceinline__ float exp2_of(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+// two fp32 values, one instruction
+struct Two { unsigned long long v; };
+__device__ __forceinline__ Two two(float a, float b) {
+    Two r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void parts(Two x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v)); }
+__device__ __forceinline__ Two operator+(Two a, Two b) {
+    Two r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Two operator*(Two a, Two b) {
+    Two r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Two multiply_add(Two a, Two b, Two c) {
+    Two r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+
+// the packet as pairs of fp32 values, and the largest of its values (NaN counts only if there is nothing else)
+__device__ __forceinline__ void pairs_of(uint4 q, Two (&z)[2], float*) {
+    z[0] = two(__uint_as_float(q.x), __uint_as_float(q.y));
+    z[1] = two(__uint_as_float(q.z), __uint_as_float(q.w));
+}
+__device__ __forceinline__ void pairs_of(uint4 q, Two (&z)[4], bf16_s*) {
+    z[0] = two(__uint_as_float(q.x << 16), __uint_as_float(q.x & 0xffff0000u));
+    z[1] = two(__uint_as_float(q.y << 16), __uint_as_float(q.y & 0xffff0000u));
+    z[2] = two(__uint_as_float(q.z << 16), __uint_as_float(q.z & 0xffff0000u));
+    z[3] = two(__uint_as_float(q.w << 16), __uint_as_float(q.w & 0xffff0000u));
+}
+__device__ __forceinline__ uint32_t max_of_pairs(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+template <int B>
+__device__ __forceinline__ float largest(const uint4 (&q)[B], float*) {
+    float m = __uint_as_float(q[0].x);
+#pragma unroll
+    for (int i = 0; i < B; ++i)
+        m = fmaxf(fmaxf(m, __uint_as_float(q[i].x)), fmaxf(fmaxf(__uint_as_float(q[i].y), __uint_as_float(q[i].z)), __uint_as_float(q[i].w)));
+    return m;
+}
+template <int B>
+__device__ __forceinline__ float largest(const uint4 (&q)[B], bf16_s*) {
+    uint32_t m = q[0].x;
+#pragma unroll
+    for (int i = 0; i < B; ++i) m = max_of_pairs(max_of_pairs(m, q[i].x), max_of_pairs(max_of_pairs(q[i].y, q[i].z), q[i].w));
+    return fmaxf(__uint_as_float(m << 16), __uint_as_float(m & 0xffff0000u));
+}
+template <typename T> __device__ __forceinline__ uint4 packet_of_minus_infinity();
+template <> __device__ __forceinline__ uint4 packet_of_minus_infinity<float>() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
+template <> __device__ __forceinline__ uint4 packet_of_minus_infinity<bf16_s>() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
+
+// (m, s, u) in units of log 2
+struct Running2 {
+    float m, s, u;
+    __device__ __forceinline__ void raise(float to) {
+        const float t = max_nan((m - to) * kLog2e, kFloor);
+        const float c = exp2_of(t);
+        u = c * (u + t * s);
+        s = c * s;
+        m = to;
+    }
+    __device__ __forceinline__ void merge(Running2 o) {
+        if (o.m > m) raise(o.m);
+        else if (m > o.m) o.raise(m);
+        s += o.s;
+        u += o.u;
+    }
+};
+
+// Keys: (ordered value, ~index), so that a larger key is a larger value or the same value at a lower index; no two entries share
+// one; 0 is no entry.
+typedef unsigned long long Key;
+__device__ __forceinline__ Key key_of(float z, int index) { return ((Key)ordered(z) << 32) | (uint32_t)~index; }
+__device__ __forceinline__ int index_of(Key k) { return (int)~(uint32_t)k; }
+__device__ __forceinline__ Key exchange(Key k, int mask) { return __shfl_xor_sync(0xffffffffu, k, mask); }
+__device__ __forceinline__ Key keep(Key mine, Key other, bool larger) { return (mine > other) == larger ? mine : other; }
+// one key a lane; descending from lane 0
+__device__ __forceinline__ Key merge_down(Key k, int lane) {
+#pragma unroll
+    for (int j = 16; j > 0; j >>= 1) k = keep(k, exchange(k, j), (lane & j) == 0);
+    return k;
+}
+__device__ __forceinline__ Key sort_down(Key k, int lane) {
+#pragma unroll
+    for (int w = 2; w <= 32; w <<= 1)
+#pragma unroll
+        for (int j = w >> 1; j > 0; j >>= 1) k = keep(k, exchange(k, j), ((lane & j) == 0) == ((lane & w) == 0 || w == 32));
+    return k;
+}
+// the 32 largest of two descending lists; b is read backwards from memory
+__device__ __forceinline__ Key join(Key a, const Key* b, int lane) {
+    const Key o = b[31 - lane];
+    return merge_down(a > o ? a : o, lane);
+}
+// The 32 largest keys of `n` (a power of two <= 2 * kWarps) descending lists in shared memory, left in list 0.
+__device__ __forceinline__ void join_lists(Key (*lists)[32], int n) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    __syncthreads();
+    for (int half = n >> 1; half > 0; half >>= 1) {
+        if (warp < half) lists[warp][lane] = join(lists[warp][lane], lists[warp + half], lane);
+        __syncthreads();
+    }
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// the same shared-memory word in CTA 0 of the cluster
+__device__ __forceinline__ uint32_t in_first_cta(const void* p) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"((uint32_t)__cvta_generic_to_shared(p)));
+    return r;
+}
+__device__ __forceinline__ void store_remote(uint32_t at, float v) { asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(at), "f"(v) : "memory"); }
+__device__ __forceinline__ void store_remote(uint32_t at, Key v) { asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(at), "l"(v) : "memory"); }
+
+constexpr int kMaxCluster = 16;
+
+// A row as the kernel walks it: `head` entries up to the 16-byte grid, whole packets, `tail` entries.
+template <typename T>
+struct RowSplit {
+    static constexpr int N = Packet<T>::N;
+    const T* z;
+    int head, tail, packets;
+    __device__ __forceinline__ RowSplit(const T* row, int vocab) : z(row) {
+        const int off = (int)(((uintptr_t)row & 15) / sizeof(T));
+        head = off ? min(N - off, vocab) : 0;
+        packets = (vocab - head) / N;
+        tail = vocab - head - packets * N;
+    }
+    __device__ __forceinline__ int first_of(int packet) const { return head + packet * N; }
+    __device__ __forceinline__ uint4 packet(int p) const { return *reinterpret_cast<const uint4*>(z + first_of(p)); }
+    // the i-th of the head + tail entries
+    __device__ __forceinline__ int edge(int i) const { return i < head ? i : i + packets * N; }
+};
+
+template <typename T>
+__device__ __forceinline__ float entry(uint4 q, int e);
+template <> __device__ __forceinline__ float entry<float>(uint4 q, int e) { return __uint_as_float(e == 0 ? q.x : e == 1 ? q.y : e == 2 ? q.z : q.w); }
+template <> __device__ __forceinline__ float entry<bf16_s>(uint4 q, int e) {
+    const uint32_t w = (e >> 1) == 0 ? q.x : (e >> 1) == 1 ? q.y : (e >> 1) == 2 ? q.z : q.w;
+    return __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
+}
+
+// The `top` largest entries of the CTA's packets [begin, end) (and, in the first CTA, of the row's edges) as a descending list in lists[0].
+// best_batch: the thread's batch whose maximum raised its own last, -1: none did (nothing but -infinity and NaN).
+template <typename T>
+__device__ __forceinline__ void top_of_slice(const RowSplit<T>& row, int begin, int end, bool edges, int top, int best_batch, Key (*lists)[32],
+                                             Key (*pending)[64]) {
+    constexpr int N = Packet<T>::N;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int n_edges = edges ? row.head + row.tail : 0;
+    // the thread's largest key: its place is looked up in the batch that holds it
+    Key mine = 0;
+    {
+        const int from = best_batch >= 0 ? best_batch : begin + tid;
+        const int until = best_batch >= 0 ? min(end, best_batch + kBatch * kThreads) : end;
+        for (int p = from; p < until; p += kThreads) {
+            const uint4 q = row.packet(p);
+#pragma unroll
+            for (int e = 0; e < N; ++e) mine = max(mine, key_of(entry<T>(q, e), row.first_of(p) + e));
+        }
+        if (tid < n_edges) mine = max(mine, key_of(widen(row.z[row.edge(tid)]), row.edge(tid)));
+    }
+    lists[warp][lane] = sort_down(mine, lane);
+    join_lists(lists, kWarps);
+    const Key tau = max(lists[0][top - 1], (Key)1);
+    const Key chosen = lane < top ? lists[0][lane] : 0;
+    __syncthreads();
+    // a warp reads every kWarps-th of the chosen groups
+    Key best = 0;
+    int waiting = 0;
+    auto offer = [&](Key k) {
+        const bool take = k >= tau;
+        const uint32_t who = __ballot_sync(0xffffffffu, take);
+        if (who == 0) return;
+        if (take) pending[warp][waiting + __popc(who & ((1u << lane) - 1))] = k;
+        waiting += __popc(who);
+        __syncwarp();
+        if (waiting >= 32) {
+            const Key k32 = sort_down(pending[warp][lane], lane);
+            const Key rest = pending[warp][32 + lane];
+            __syncwarp();
+            pending[warp][lane] = rest;
+            const Key other = __shfl_sync(0xffffffffu, k32, 31 - lane);
+            best = merge_down(best > other ? best : other, lane);
+            waiting -= 32;
+            __syncwarp();
+        }
+    };
+    for (int g = warp; g < top; g += kWarps) {
+        const Key k = __shfl_sync(0xffffffffu, chosen, g);
+        if (k == 0) break;
+        const int index = index_of(k);
+        const bool at_edge = index < row.head || index >= row.head + row.packets * N;
+        const int who = at_edge ? (index < row.head ? index : index - row.packets * N) : ((index - row.head) / N - begin) % kThreads;
+        for (int p0 = begin + who; p0 < end; p0 += 32 * kThreads) {
+            const int p = p0 + lane * kThreads;
+            const bool there = p < end;
+            uint4 q = packet_of_minus_infinity<T>();
+            if (there) q = row.packet(p);
+#pragma unroll
+            for (int e = 0; e < N; ++e) offer(there ? key_of(entry<T>(q, e), row.first_of(p) + e) : 0);
+        }
+        if (who < n_edges) offer(lane == 0 ? key_of(widen(row.z[row.edge(who)]), row.edge(who)) : 0);
+    }
+    {
+        const Key k32 = sort_down(lane < waiting ? pending[warp][lane] : 0, lane);
+        const Key other = __shfl_sync(0xffffffffu, k32, 31 - lane);
+        best = merge_down(best > other ? best : other, lane);
+    }
+    lists[warp][lane] = best;
+    join_lists(lists, kWarps);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads) logprobs_kernel(const T* __restrict__ logits, long long ld, long long rows, int vocab,
+                                                            const int* __restrict__ tokens, float* __restrict__ logprob,
+                                                            float* __restrict__ entropy, float* __restrict__ lse_out, int top,
+                                                            float* __restrict__ top_logprobs, int* __restrict__ top_tokens, int cluster) {
+    constexpr int N = Packet<T>::N;
+    __shared__ Running2 sm[kWarps];
+    __shared__ Running2 from_cta[kMaxCluster];
+    __shared__ Key lists[kMaxCluster][32];
+    __shared__ Key pending[kWarps][64];
+    __shared__ Key from_cta_keys[kMaxCluster][32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int rank = cluster > 1 ? (int)cluster_rank() : 0;
+    if (cluster > 1) cluster_arrive();          // every CTA of the cluster runs before its shared memory is written from another
+    dependent_prologue();
+    bool started = cluster == 1;
+    for (long long r = blockIdx.x / cluster; r < rows; r += gridDim.x / cluster) {
+        const RowSplit<T> row(logits + r * ld, vocab);
+        const int share = (row.packets + cluster - 1) / cluster;
+        const int begin = min(row.packets, rank * share), end = min(row.packets, begin + share);
+        Running2 me = {Lowest<float>::value(), 0, 0};
+        float seen = -infinity_of(0.0f);
+        int best_batch = -1;
+        {
+            Two s2 = two(0, 0), u2 = two(0, 0);
+            auto raise = [&](float to) {
+                float a, b, c, d;
+                parts(s2, a, b);
+                parts(u2, c, d);
+                me.s = a + b;
+                me.u = c + d;
+                me.raise(to);
+                s2 = two(me.s, 0);
+                u2 = two(me.u, 0);
+            };
+            for (int b = begin + tid; b < end; b += kBatch * kThreads) {
+                uint4 q[kBatch];
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) q[i] = b + i * kThreads < end ? row.packet(b + i * kThreads) : packet_of_minus_infinity<T>();
+                const float high = largest(q, (T*)nullptr);
+                if (high > seen) {
+                    seen = high;
+                    best_batch = b;
+                    if (high > me.m) raise(high);
+                }
+                const Two minus = two(-me.m, -me.m), scale = two(kLog2e, kLog2e);
+#pragma unroll
+                for (int i = 0; i < kBatch; ++i) {
+                    Two z[N / 2];
+                    pairs_of(q[i], z, (T*)nullptr);
+#pragma unroll
+                    for (int e = 0; e < N / 2; ++e) {
+                        float t0, t1;
+                        parts((z[e] + minus) * scale, t0, t1);
+                        t0 = max_nan(t0, kFloor);
+                        t1 = max_nan(t1, kFloor);
+                        const Two p = two(exp2_of(t0), exp2_of(t1));
+                        s2 = s2 + p;
+                        u2 = multiply_add(two(t0, t1), p, u2);
+                    }
+                }
+            }
+            if (rank == 0 && tid < row.head + row.tail) {
+                const float z = widen(row.z[row.edge(tid)]);
+                if (z > me.m) raise(z);
+                const float t = max_nan((z - me.m) * kLog2e, kFloor), p = exp2_of(t);
+                s2 = s2 + two(p, 0);
+                u2 = u2 + two(t * p, 0);
+            }
+            raise(me.m);
+        }
+#pragma unroll
+        for (int m = 16; m > 0; m >>= 1) {
+            Running2 o;
+            o.m = __shfl_xor_sync(0xffffffffu, me.m, m);
+            o.s = __shfl_xor_sync(0xffffffffu, me.s, m);
+            o.u = __shfl_xor_sync(0xffffffffu, me.u, m);
+            me.merge(o);
+        }
+        __syncthreads();          // the row before has been written
+        if (lane == 0) sm[warp] = me;
+        if (top > 0) top_of_slice(row, begin, end, rank == 0, top, best_batch, lists, pending);
+        else __syncthreads();
+        if (cluster > 1) {
+            if (!started) { cluster_wait(); started = true; }
+            if (warp == 0) {
+                if (lane == 0) {
+                    Running2 all = sm[0];
+#pragma unroll
+                    for (int w = 1; w < kWarps; ++w) all.merge(sm[w]);
+                    store_remote(in_first_cta(&from_cta[rank].m), all.m);
+                    store_remote(in_first_cta(&from_cta[rank].s), all.s);
+                    store_remote(in_first_cta(&from_cta[rank].u), all.u);
+                }
+                if (top > 0) store_remote(in_first_cta(&from_cta_keys[rank][lane]), lists[0][lane]);
+            }
+            cluster_arrive();
+            cluster_wait();
+            if (rank == 0 && top > 0) {
+                for (int w = warp; w < cluster; w += kWarps) lists[w][lane] = from_cta_keys[w][lane];
+                join_lists(lists, cluster);
+            }
+        }
+        if (rank == 0 && warp == 0) {
+            Running2 all = cluster > 1 ? from_cta[0] : sm[0];
+            for (int w = 1; w < (cluster > 1 ? cluster : kWarps); ++w) all.merge(cluster > 1 ? from_cta[w] : sm[w]);
+            float l, h;
+            if (all.s == 0) {          // nothing but -infinity
+                l = -infinity_of(0.0f);
+                h = 0;
+            } else {
+                const float ls = logf(all.s);
+                l = all.m + ls;
+                h = ls - kLn2 * (all.u / all.s);
+            }
+            if (lane == 0) {
+                if (entropy) entropy[r] = h;
+                if (lse_out) lse_out[r] = l;
+                if (logprob) {
+                    const int t = tokens[r];
+                    logprob[r] = t < 0 ? 0.0f : t >= vocab ? nan_of(0.0f) : log_p(widen(row.z[t]), l);
+                }
+            }
+            if (lane < top) {
+                const int index = index_of(lists[0][lane]);
+                top_tokens[r * top + lane] = index;
+                top_logprobs[r * top + lane] = log_p(widen(row.z[index]), l);
+            }
+        }
+        if (cluster > 1) {           // the first CTA has read what the others sent for this row
+            cluster_arrive();
+            cluster_wait();
+        }
+    }
+    if (!started) cluster_wait();
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kThreads) logprobs_backward_kernel(const T* logits, long long ld, long long rows, int vocab,
                                                                      const int* __restrict__ tokens,
@@ -216,10 +601,32 @@ long long capped(long long want, long long most) { return std::max<long long>(1,
 template <typename T>
 cudaError_t forward(cudaStream_t s, const Rows& z, const int* tokens, void* logprob, void* entropy, void* lse, int top, void* top_logprobs,
                     int* top_tokens) {
-    typedef typename AccOf<T>::type A;
-    return launch(logprobs_rows_kernel<T>, dim3((unsigned)capped(z.rows, kSms * 64)), kThreads, 0, s, 1, (const T*)z.data,
-                  (long long)z.stride, (long long)z.rows, (int)z.cols, tokens, (A*)logprob, (A*)entropy, (A*)lse, top, (A*)top_logprobs,
-                  top_tokens);
+    // as many CTAs a row as fill the machine, none with less than one batch of packets for its threads
+    const long long packets = z.cols / Packet<T>::N;
+    int cluster = 1;
+    while (cluster < kMaxCluster && z.rows * cluster < kSms * 8 && packets >= 2ll * cluster * kBatch * kThreads) cluster *= 2;
+    if (cluster > 8) {
+        static std::atomic<unsigned long long> allowed(0);      // by device
+        int device = 0;
+        cudaError_t e = cudaGetDevice(&device);
+        if (e == cudaSuccess && !(allowed.load() >> (device & 63) & 1)) {
+            e = cudaFuncSetAttribute(logprobs_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+            if (e == cudaSuccess) allowed.fetch_or(1ull << (device & 63));
+        }
+        if (e != cudaSuccess) return e;
+    }
+    const long long clusters = std::min<long long>(z.rows, (1ll << 30) / cluster);
+    return launch(logprobs_kernel<T>, dim3((unsigned)(clusters * cluster)), kThreads, 0, s, cluster, (const T*)z.data, (long long)z.stride,
+                  (long long)z.rows, (int)z.cols, tokens, (float*)logprob, (float*)entropy, (float*)lse, top, (float*)top_logprobs, top_tokens,
+                  cluster);
+}
+
+template <>
+cudaError_t forward<double>(cudaStream_t s, const Rows& z, const int* tokens, void* logprob, void* entropy, void* lse, int top,
+                            void* top_logprobs, int* top_tokens) {
+    return launch(logprobs_rows_kernel<double>, dim3((unsigned)capped(z.rows, kSms * 64)), kThreads, 0, s, 1, (const double*)z.data,
+                  (long long)z.stride, (long long)z.rows, (int)z.cols, tokens, (double*)logprob, (double*)entropy, (double*)lse, top,
+                  (double*)top_logprobs, top_tokens);
 }
 
 template <typename T>
