@@ -8,6 +8,7 @@
 // The backward pass takes x and no saved statistics: it has to read x anyway, and mean and r of a row that is at hand cost
 // no memory traffic.  Statistics and sums are held in fp32 (fp64 for fp64 rows).
 #include <algorithm>
+#include <atomic>
 
 #include "op_device.cuh"
 #include "op_host.h"
@@ -143,6 +144,430 @@ __global__ void __launch_bounds__(kThreads) fold_columns_kernel(const A* __restr
     }
 }
 
+// ---------------------------------------------------------------------------------------------- rows held in registers
+// f32 and bf16 rows that fit: some warps share a row, a thread keeps packets of it.  Statistics need one exchange between the warps: each warp takes its own mean first (shuffles), then
+//   Q = sum (x - mean_w)^2,  A = sum a,  C = sum a (x - mean_w)
+// about it, and the warps' values are moved to the row's mean as they are added:
+//   sum (x - mean)^2 = sum_w Q_w + n_w (mean_w - mean)^2,   sum a (x - mean) = sum_w C_w + A_w (mean_w - mean).
+// No squares of values far from zero are subtracted from one another, and the backward pass needs no more exchanges with
+// recomputed statistics than it would with saved ones.
+
+// A thread holds C packets of W elements of a row, the row's WR warps side by side (W = 1: rows that are off the 16-byte grid or no
+// whole number of 16-byte packets).  Whole packets come through a ring of DEPTH rows in shared memory that every thread
+// fills and reads for itself (cp.async; no thread waits for another one's copies), so that the loads of the next rows are under way
+// while a row is worked on.
+// FULL: every thread of the row holds all C of them.
+template <int W, int C, int WR, bool FULL>
+struct Held {
+    uint32_t there;          // bit i: the thread's i-th packet is one of the row's
+    int first;               // column of the first packet; the others lie 32 WR W columns apart
+    int mine;                // elements that this warp holds
+    __device__ __forceinline__ Held(int t, int cols) : there(0), first(t * W), mine(of_warp(t >> 5, cols)) {
+#pragma unroll
+        for (int i = 0; i < C; ++i)
+            if (column(i) < cols) there |= 1u << i;
+    }
+    __device__ __forceinline__ int column(int i) const { return first + i * 32 * WR * W; }
+    __device__ __forceinline__ bool has(int i) const { return FULL || (there >> i & 1); }
+    static __device__ __forceinline__ int of_warp(int w, int cols) {
+        if (FULL) return 32 * C * W;
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < C; ++i) n += min(max(cols / W - (i * WR + w) * 32, 0), 32) * W;
+        return n;
+    }
+};
+
+__device__ __forceinline__ void copy_async(uint4* to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copies_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void copies_but() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// W neighbouring values: pairs, which one instruction works on, or a single one.
+template <int W>
+struct Vals {
+    Two p[W / 2];
+    __device__ __forceinline__ void all(float a) {
+#pragma unroll
+        for (int e = 0; e < W / 2; ++e) p[e] = both(a);
+    }
+    __device__ __forceinline__ float sum() const {
+        Two s = p[0];
+#pragma unroll
+        for (int e = 1; e < W / 2; ++e) s = s + p[e];
+        return total(s);
+    }
+    __device__ __forceinline__ void add(float a) {
+#pragma unroll
+        for (int e = 0; e < W / 2; ++e) p[e] = p[e] + both(a);
+    }
+    __device__ __forceinline__ void add(const Vals& a) {
+#pragma unroll
+        for (int e = 0; e < W / 2; ++e) p[e] = p[e] + a.p[e];
+    }
+    __device__ __forceinline__ void mul(float a) {
+#pragma unroll
+        for (int e = 0; e < W / 2; ++e) p[e] = p[e] * both(a);
+    }
+    __device__ __forceinline__ void mul(const Vals& a) {
+#pragma unroll
+        for (int e = 0; e < W / 2; ++e) p[e] = p[e] * a.p[e];
+    }
+    __device__ __forceinline__ void fma(const Vals& a, const Vals& b, const Vals& c) {        // a b + c
+#pragma unroll
+        for (int e = 0; e < W / 2; ++e) p[e] = multiply_add(a.p[e], b.p[e], c.p[e]);
+    }
+    __device__ __forceinline__ void fma(const Vals& a, const Vals& b, float c) {
+#pragma unroll
+        for (int e = 0; e < W / 2; ++e) p[e] = multiply_add(a.p[e], b.p[e], both(c));
+    }
+    __device__ __forceinline__ void fma(const Vals& a, float b, const Vals& c) {
+#pragma unroll
+        for (int e = 0; e < W / 2; ++e) p[e] = multiply_add(a.p[e], both(b), c.p[e]);
+    }
+    __device__ __forceinline__ float value(int e) const {
+        float a, b;
+        parts(p[e / 2], a, b);
+        return e & 1 ? b : a;
+    }
+    template <typename T> __device__ __forceinline__ void read(const T* from) { pairs_of(*reinterpret_cast<const uint4*>(from), p, from); }
+    template <typename T> __device__ __forceinline__ void write(T* to) const { *reinterpret_cast<uint4*>(to) = packet_of(p, to); }
+    // weights: W values of any type that lie on the 16-byte grid
+    __device__ __forceinline__ void weights(const float* w) {
+#pragma unroll
+        for (int i = 0; i < W / 4; ++i) {
+            const float4 q = reinterpret_cast<const float4*>(w)[i];
+            p[2 * i] = two(q.x, q.y);
+            p[2 * i + 1] = two(q.z, q.w);
+        }
+    }
+    __device__ __forceinline__ void weights(const bf16_s* w) { read(w); }
+};
+template <>
+struct Vals<1> {
+    float f;
+    __device__ __forceinline__ void all(float a) { f = a; }
+    __device__ __forceinline__ float sum() const { return f; }
+    __device__ __forceinline__ void add(float a) { f += a; }
+    __device__ __forceinline__ void add(const Vals& a) { f += a.f; }
+    __device__ __forceinline__ void mul(float a) { f *= a; }
+    __device__ __forceinline__ void mul(const Vals& a) { f *= a.f; }
+    __device__ __forceinline__ void fma(const Vals& a, const Vals& b, const Vals& c) { f = __fmaf_rn(a.f, b.f, c.f); }
+    __device__ __forceinline__ void fma(const Vals& a, const Vals& b, float c) { f = __fmaf_rn(a.f, b.f, c); }
+    __device__ __forceinline__ void fma(const Vals& a, float b, const Vals& c) { f = __fmaf_rn(a.f, b, c.f); }
+    __device__ __forceinline__ float value(int) const { return f; }
+    template <typename T> __device__ __forceinline__ void read(const T* from) { f = widen(*from); }
+    template <typename T> __device__ __forceinline__ void write(T* to) const { *to = Narrow<T>::of(f); }
+    template <typename T> __device__ __forceinline__ void weights(const T* w) { f = widen(*w); }
+};
+
+// over WR neighbouring lanes
+template <int WR>
+__device__ __forceinline__ float sum_of(float v) {
+#pragma unroll
+    for (int m = WR / 2; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+    return v;
+}
+
+// s / n, from 1 / n and one correction
+__device__ __forceinline__ float quotient(float s, int n, float per_n) {
+    const float m = s * per_n;
+    return __fmaf_rn(__fmaf_rn(-m, (float)n, s), per_n, m);
+}
+
+// The threads that share a row meet: at most four groups of a CTA, each at a barrier of its own.  (A barrier whose number is
+// computed would count as all sixteen.)
+template <int WR, int GROUPS>
+__device__ __forceinline__ void row_barrier(int group) {
+    if (GROUPS == 1) __syncthreads();
+    else if (group == 0) asm volatile("bar.sync 1, %0;" ::"n"(32 * WR) : "memory");
+    else if (group == 1) asm volatile("bar.sync 2, %0;" ::"n"(32 * WR) : "memory");
+    else if (group == 2) asm volatile("bar.sync 3, %0;" ::"n"(32 * WR) : "memory");
+    else asm volatile("bar.sync 4, %0;" ::"n"(32 * WR) : "memory");
+}
+
+template <typename T, typename P, int W, int C, int WR, int GROUPS, int DEPTH, int CTAS, bool FULL>
+__global__ void __launch_bounds__(32 * WR * GROUPS, CTAS) norm_resident_kernel(const T* x, long long ldx, const P* __restrict__ gamma,
+                                                                               const P* __restrict__ beta, T* y, long long ldy,
+                                                                               long long rows, int cols, float eps) {
+    constexpr int THREADS = 32 * WR * GROUPS;
+    extern __shared__ uint4 ring[];          // [DEPTH][C][THREADS]
+    __shared__ float2 sm[2][GROUPS * WR];
+    dependent_prologue();
+    const int lane = threadIdx.x & 31, group = threadIdx.x / (32 * WR), warp = threadIdx.x / 32 % WR;
+    const Held<W, C, WR, FULL> at(threadIdx.x % (32 * WR), cols);
+    const float per_mine = at.mine ? 1.0f / at.mine : 0.0f, per_col = 1.0f / cols;
+    const float its = Held<W, C, WR, FULL>::of_warp(lane % WR, cols), per_its = its ? 1.0f / its : 0.0f;      // of the warp whose sums this lane looks after
+    const long long step = (long long)gridDim.x * GROUPS;
+    long long row = (long long)blockIdx.x * GROUPS + group;
+    // The weights stay in registers where there are not too many of them: reading them again for every row, 32 bytes for each 16 of
+    // a bf16 row, kept L1 85% busy at 40% of the memory's bandwidth (62 us instead of 43 for 16384 x 4096).
+    constexpr bool HOLD = C * W <= 16;
+    Vals<W> g[HOLD ? C : 1], b[HOLD ? C : 1];
+    if (HOLD) {
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            g[i].all(1);
+            b[i].all(0);
+            if (gamma && at.has(i)) g[i].weights(gamma + at.column(i));
+            if (beta && at.has(i)) b[i].weights(beta + at.column(i));
+        }
+    }
+    const T *from = x + row * ldx, *ahead = from;          // the row, and the next one to be fetched
+    T* to = y + row * ldy;
+    long long fetched = row;
+    auto fetch = [&](int stage) {
+        if (fetched < rows) {
+#pragma unroll
+            for (int i = 0; i < C; ++i)
+                if (at.has(i)) copy_async(ring + (stage * C + i) * THREADS + threadIdx.x, ahead + at.column(i));
+        }
+        copies_issued();
+        fetched += step;
+        ahead += step * ldx;
+    };
+    if (W > 1)
+        for (int d = 0; d < DEPTH - 1; ++d) fetch(d);
+    int stage = 0, turn = 0;
+    for (; row < rows; row += step, from += step * ldx, to += step * ldy) {
+        if (W > 1) {
+            fetch(stage ? stage - 1 : DEPTH - 1);
+            copies_but<DEPTH - 1>();
+        }
+        Vals<W> v[C];
+        float sum = 0;
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+            if (at.has(i)) v[i].read(W > 1 ? (const T*)(ring + (stage * C + i) * THREADS + threadIdx.x) : from + at.column(i));
+            else v[i].all(0);
+            sum += v[i].sum();
+        }
+        sum = warp_sum(sum);
+        const float mean_w = sum * per_mine;
+        Vals<W> squares;
+        squares.all(0);
+#pragma unroll
+        for (int i = 0; i < C; ++i)
+            if (at.has(i)) {
+                Vals<W> d = v[i];
+                d.add(-mean_w);
+                squares.fma(d, d, squares);
+            }
+        float q = warp_sum(squares.sum());
+        float mean = quotient(sum, cols, per_col);
+        if (WR > 1) {
+            float2* all = sm[turn] + group * WR;
+            turn ^= 1;
+            if (lane == 0) all[warp] = make_float2(sum, q);
+            row_barrier<WR, GROUPS>(group);
+            const float2 o = all[lane % WR];
+            mean = quotient(sum_of<WR>(o.x), cols, per_col);
+            const float d = o.x * per_its - mean;
+            q = sum_of<WR>(o.y + its * d * d);
+        }
+        const float r = rsqrtf(q * per_col + eps);
+#pragma unroll
+        for (int i = 0; i < C; ++i)
+            if (at.has(i)) {
+                v[i].add(-mean);          // (exact for a row that does not vary, where r is largest)
+                v[i].mul(r);
+                if (HOLD) {
+                    v[i].fma(v[i], g[i], b[i]);
+                } else {
+                    Vals<W> w;
+                    if (gamma) {
+                        w.weights(gamma + at.column(i));
+                        v[i].mul(w);
+                    }
+                    if (beta) {
+                        w.weights(beta + at.column(i));
+                        v[i].add(w);
+                    }
+                }
+                v[i].write(to + at.column(i));
+            }
+        stage = stage + 1 == DEPTH ? 0 : stage + 1;
+    }
+}
+
+// Every CTA takes rows gridDim.x * GROUPS apart, sums dy h and dy of its columns in registers and leaves them, its groups added in
+// their order, in partial[CTA][0 / 1].
+template <typename T, typename P, int W, int C, int WR, int GROUPS, int DEPTH, int CTAS, bool FULL>
+__global__ void __launch_bounds__(32 * WR * GROUPS, CTAS)
+    norm_backward_resident_kernel(const T* dy, long long lddy, const T* x, long long ldx, const P* __restrict__ gamma, T* dx, long long lddx,
+                                  long long rows, int cols, float eps, float* __restrict__ partial) {
+    constexpr int THREADS = 32 * WR * GROUPS;
+    extern __shared__ uint4 ring[];          // [DEPTH][2][C][THREADS]; in the end [2][cols] sums, where several groups have some to add
+    __shared__ float4 sm[2][GROUPS * WR];
+    dependent_prologue();
+    const int lane = threadIdx.x & 31, group = threadIdx.x / (32 * WR), warp = threadIdx.x / 32 % WR;
+    const Held<W, C, WR, FULL> at(threadIdx.x % (32 * WR), cols);
+    const float per_mine = at.mine ? 1.0f / at.mine : 0.0f, per_col = 1.0f / cols;
+    const float its = Held<W, C, WR, FULL>::of_warp(lane % WR, cols), per_its = its ? 1.0f / its : 0.0f;      // of the warp whose sums this lane looks after
+    const long long step = (long long)gridDim.x * GROUPS;
+    long long row = (long long)blockIdx.x * GROUPS + group;
+    // Up to 16 values a thread, the row and its weights stay in registers across the exchange; above, they are read again behind it
+    // (the row from the ring, the weights from L1), and the sums of the columns have the registers.
+    constexpr bool HOLD = C * W <= 16;
+    constexpr int H = HOLD ? C : 1;
+    Vals<W> g[H], dg[C], db[C];
+    auto weigh = [&](int i) {
+        g[HOLD ? i : 0].all(1);
+        if (gamma && at.has(i)) g[HOLD ? i : 0].weights(gamma + at.column(i));
+    };
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+        dg[i].all(0);
+        db[i].all(0);
+        if (HOLD) weigh(i);
+    }
+    auto slot = [&](int stage, int which, int i) { return ring + ((stage * 2 + which) * C + i) * THREADS + threadIdx.x; };
+    const T *from_x = x + row * ldx, *from_dy = dy + row * lddy, *ahead_x = from_x, *ahead_dy = from_dy;
+    T* to_dx = dx + row * lddx;
+    long long fetched = row;
+    auto fetch = [&](int stage) {
+        if (fetched < rows) {
+#pragma unroll
+            for (int i = 0; i < C; ++i)
+                if (at.has(i)) {
+                    copy_async(slot(stage, 0, i), ahead_x + at.column(i));
+                    copy_async(slot(stage, 1, i), ahead_dy + at.column(i));
+                }
+        }
+        copies_issued();
+        fetched += step;
+        ahead_x += step * ldx;
+        ahead_dy += step * lddy;
+    };
+    if (W > 1)
+        for (int d = 0; d < DEPTH - 1; ++d) fetch(d);
+    int stage = 0, turn = 0;
+    for (; row < rows; row += step, from_x += step * ldx, from_dy += step * lddy, to_dx += step * lddx) {
+        if (W > 1) {
+            fetch(stage ? stage - 1 : DEPTH - 1);
+            copies_but<DEPTH - 1>();
+        }
+        Vals<W> v[H], u[H];
+        float sum = 0;
+        auto read_x = [&](int i) { v[HOLD ? i : 0].read(W > 1 ? (const T*)slot(stage, 0, i) : from_x + at.column(i)); };
+        auto read_dy = [&](int i) { u[HOLD ? i : 0].read(W > 1 ? (const T*)slot(stage, 1, i) : from_dy + at.column(i)); };
+#pragma unroll
+        for (int i = 0; i < C; ++i)
+            if (at.has(i)) {
+                read_x(i);
+                if (HOLD) read_dy(i);
+                sum += v[HOLD ? i : 0].sum();
+            }
+        sum = warp_sum(sum);
+        const float mean_w = sum * per_mine;
+        Vals<W> sq, sa, sc;
+        sq.all(0);
+        sa.all(0);
+        sc.all(0);
+#pragma unroll
+        for (int i = 0; i < C; ++i)
+            if (at.has(i)) {
+                const int k = HOLD ? i : 0;
+                if (!HOLD) {
+                    read_x(i);
+                    read_dy(i);
+                    weigh(i);
+                }
+                Vals<W> d = v[k], ae = u[k];
+                d.add(-mean_w);
+                ae.mul(g[k]);
+                sq.fma(d, d, sq);
+                sa.add(ae);
+                sc.fma(ae, d, sc);
+            }
+        float q = warp_sum(sq.sum()), a = warp_sum(sa.sum()), c = warp_sum(sc.sum());
+        float mean = quotient(sum, cols, per_col);
+        if (WR > 1) {
+            float4* all = sm[turn] + group * WR;
+            turn ^= 1;
+            if (lane == 0) all[warp] = make_float4(sum, q, a, c);
+            row_barrier<WR, GROUPS>(group);
+            const float4 o = all[lane % WR];
+            mean = quotient(sum_of<WR>(o.x), cols, per_col);
+            const float d = o.x * per_its - mean;      // (a warp without elements has o.x = o.z = 0)
+            q = sum_of<WR>(o.y + its * d * d);
+            a = sum_of<WR>(o.z);
+            c = sum_of<WR>(o.w + o.z * d);
+        }
+        const float r = rsqrtf(q * per_col + eps);
+        const float c1 = -r * (a * per_col), c2 = -r * r * (r * (c * per_col));
+#pragma unroll
+        for (int i = 0; i < C; ++i)
+            if (at.has(i)) {
+                const int k = HOLD ? i : 0;
+                if (!HOLD) {
+                    read_x(i);
+                    read_dy(i);
+                    weigh(i);
+                }
+                v[k].add(-mean);          // h / r
+                db[i].add(u[k]);
+                u[k].mul(r);
+                dg[i].fma(u[k], v[k], dg[i]);
+                u[k].fma(u[k], g[k], c1);
+                u[k].fma(v[k], c2, u[k]);
+                if (dx) u[k].write(to_dx + at.column(i));
+            }
+        stage = stage + 1 == DEPTH ? 0 : stage + 1;
+    }
+    if (!partial) return;
+    float* to = partial + 2 * (long long)blockIdx.x * cols;
+    float* columns = reinterpret_cast<float*>(ring);
+    if (GROUPS > 1) __syncthreads();          // the ring is done with
+    for (int k = 0; k < GROUPS; ++k) {
+        if (group == k) {
+#pragma unroll
+            for (int i = 0; i < C; ++i)
+                if (at.has(i)) {
+#pragma unroll
+                    for (int e = 0; e < W; ++e) {
+                        float *pg = (GROUPS == 1 ? to : columns) + at.column(i) + e, *pb = pg + cols;
+                        *pg = k ? *pg + dg[i].value(e) : dg[i].value(e);
+                        *pb = k ? *pb + db[i].value(e) : db[i].value(e);
+                    }
+                }
+        }
+        if (GROUPS > 1) __syncthreads();
+    }
+    if (GROUPS > 1)
+        for (int i = threadIdx.x; i < 2 * cols; i += THREADS) to[i] = columns[i];
+}
+
+// How rows are held: `packets` a thread, `warps` a row (0: they are too long), rows a CTA at a time where a row has fewer than 8 warps.
+struct Layout { int packets, warps; };
+constexpr int groups_of(int warps) { return warps < 8 ? 8 / warps : 1; }
+
+// Forward, measured at 2^26 elements: 16 values a thread (16384 x 4096 bf16: 43 us; 8 values 53, 32 values 58), 8 where a warp can hold
+// the row with them (65536 x 256 f32: 23 us; two warps 23 to 29), 32 for rows that 8 warps cannot hold with 16.
+Layout forward_layout(int size, int64_t cols) {
+    const int64_t packets = (cols + 16 / size - 1) / (16 / size);
+    Layout l = {size == 2 ? 2 : 4, 1};
+    if (packets <= 32ll * l.packets / 2) l.packets /= 2;
+    else if (size == 2 && packets > 32 * 8 * 2) l.packets = 4;
+    while (l.warps <= 32 && 32ll * l.packets * l.warps < packets) l.warps *= 2;
+    if (l.warps > 32) l.warps = 0;
+    return l;
+}
+// Backward: 16 values a thread for bf16 rows (16384 x 4096: 82 us; 8 values 103), 8 for f32 rows (65536 x 1024: 127 us; 16 values 144);
+// 32 for rows that 16 warps cannot hold with these.
+Layout backward_layout(int size, int64_t cols) {
+    const int64_t packets = (cols + 16 / size - 1) / (16 / size);
+    Layout l = {size == 2 && packets <= 32 ? 1 : 2, 1};
+    while (l.warps <= 16 && 32ll * l.packets * l.warps < packets) l.warps *= 2;
+    if (l.warps > 16) l = {size == 2 ? 4 : 8, 32ll * 16 * (size == 2 ? 4 : 8) < packets ? 0 : 16};
+    return l;
+}
+bool on_grid(const void* p) { return (uintptr_t)p % 16 == 0; }
+bool on_grid(const Rows& m) {
+    return (uintptr_t)m.data % 16 == 0 && m.cols % (16 / m.size) == 0 && (m.rows < 2 || m.stride % (16 / m.size) == 0);
+}
+
 long long capped(long long want, long long most) { return std::max<long long>(1, std::min(want, most)); }
 
 long long column_slices(long long rows, long long cols) {
@@ -150,29 +575,141 @@ long long column_slices(long long rows, long long cols) {
     return capped((kSms * 8 + tiles - 1) / tiles, std::max<long long>(1, rows / 4));
 }
 
+// A CTA that holds 16 values a thread in 256 threads takes half of an SM's registers.
+long long backward_ctas(const Layout& l, int64_t rows) {
+    const int groups = groups_of(l.warps);
+    return capped((rows + groups - 1) / groups, kSms * (l.warps > 8 ? 1 : 2));
+}
+
 struct BackwardSpace { size_t stats, partial, total; long long slices; };
 BackwardSpace backward_space(int dtype, int64_t rows, int64_t cols) {
     const size_t a = dtype == DALIB200_F64 ? 8 : 4;
     BackwardSpace b;
-    b.slices = column_slices(rows, cols);
-    b.stats = ((size_t)rows * 4 * a + 255) / 256 * 256;
+    const Layout l = backward_layout(size_of(dtype), cols);
+    if (dtype != DALIB200_F64 && l.warps) {
+        b.slices = backward_ctas(l, rows);
+        b.stats = 0;
+    } else {
+        b.slices = column_slices(rows, cols);
+        b.stats = ((size_t)rows * 4 * a + 255) / 256 * 256;
+    }
     b.partial = (size_t)b.slices * 2 * cols * a;
     b.total = b.stats + b.partial;
     return b;
 }
 
+// Lets the kernel take more shared memory than every kernel may; asked for once a device (`done`: a bit for each).
+template <typename K>
+cudaError_t allow_shared(K kernel, size_t bytes, std::atomic<unsigned long long>* done) {
+    if (bytes <= 40 * 1024) return cudaSuccess;
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess || done->load() >> (device & 63) & 1) return e;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess) done->fetch_or(1ull << (device & 63));
+    return e;
+}
+
+constexpr int kDepth = 3;
+template <typename T, typename P, int C, int WR>
+cudaError_t forward_resident(cudaStream_t s, const Rows& x, const void* gamma, const void* beta, const Rows& y, double eps) {
+    constexpr int N = Packet<T>::N, GROUPS = groups_of(WR), THREADS = 32 * WR * GROUPS;
+    constexpr int CTAS = THREADS == 256 ? (C * N > 16 ? 2 : C * N > 8 ? 3 : 4) : THREADS == 512 ? (C * N > 8 ? 1 : 2) : 1;
+    const bool vec = on_grid(x) && on_grid(y) && on_grid(gamma) && on_grid(beta);
+    const bool full = vec && x.cols == (int64_t)32 * WR * C * N;
+    auto kernel = full  ? norm_resident_kernel<T, P, N, C, WR, GROUPS, kDepth, CTAS, true>
+                  : vec ? norm_resident_kernel<T, P, N, C, WR, GROUPS, kDepth, CTAS, false>
+                        : norm_resident_kernel<T, P, 1, C * N, WR, GROUPS, kDepth, CTAS, false>;
+    const size_t smem = vec ? (size_t)kDepth * C * THREADS * 16 : 0;
+    static std::atomic<unsigned long long> allowed[2];
+    const cudaError_t e = allow_shared(kernel, smem, &allowed[full]);
+    if (e != cudaSuccess) return e;
+    const long long ctas = (x.rows + GROUPS - 1) / GROUPS;
+    return launch(kernel, dim3((unsigned)capped(ctas, kSms * (vec ? CTAS : 32))), THREADS, smem, s, 1,
+                  (const T*)x.data, (long long)x.stride, (const P*)gamma, (const P*)beta, (T*)y.data, (long long)y.stride,
+                  (long long)x.rows, (int)x.cols, (float)eps);
+}
+template <typename T, typename P, int C>
+cudaError_t forward_resident(cudaStream_t s, int warps, const Rows& x, const void* gamma, const void* beta, const Rows& y, double eps) {
+    switch (warps) {
+        case 1: return forward_resident<T, P, C, 1>(s, x, gamma, beta, y, eps);
+        case 2: return forward_resident<T, P, C, 2>(s, x, gamma, beta, y, eps);
+        case 4: return forward_resident<T, P, C, 4>(s, x, gamma, beta, y, eps);
+        case 8: return forward_resident<T, P, C, 8>(s, x, gamma, beta, y, eps);
+        case 16: return forward_resident<T, P, C, 16>(s, x, gamma, beta, y, eps);
+        default: return forward_resident<T, P, C, 32>(s, x, gamma, beta, y, eps);
+    }
+}
+
 template <typename T, typename P>
 cudaError_t forward(cudaStream_t s, const Rows& x, const void* gamma, const void* beta, const Rows& y, double eps) {
+    if constexpr (sizeof(T) < 8) {
+        const Layout l = forward_layout(sizeof(T), x.cols);
+        constexpr int C = sizeof(T) == 2 ? 1 : 2;
+        if (l.warps)
+            return l.packets == C       ? forward_resident<T, P, C, 1>(s, x, gamma, beta, y, eps)
+                   : l.packets == 2 * C ? forward_resident<T, P, 2 * C>(s, l.warps, x, gamma, beta, y, eps)
+                                        : forward_resident<T, P, 4>(s, l.warps, x, gamma, beta, y, eps);
+    }
     return launch(norm_rows_kernel<T, P>, dim3((unsigned)capped(x.rows, kSms * 64)), kThreads, 0, s, 1, (const T*)x.data,
                   (long long)x.stride, (const P*)gamma, (const P*)beta, (T*)y.data, (long long)y.stride, (long long)x.rows,
                   (long long)x.cols, eps);
+}
+
+template <typename P, typename A>
+cudaError_t fold_columns(cudaStream_t s, const A* partial, long long slices, long long cols, void* dgamma, void* dbeta) {
+    return launch(fold_columns_kernel<A, P>, dim3((unsigned)((cols + 31) / 32), 2), kThreads, 0, s, 1, partial, slices, cols, (P*)dgamma,
+                  (P*)dbeta);
+}
+
+template <typename T, typename P, int C, int WR>
+cudaError_t backward_resident(cudaStream_t s, const BackwardSpace& b, const Rows& dy, const Rows& x, const void* gamma, const Rows& dx,
+                              void* dgamma, void* dbeta, double eps, void* space) {
+    constexpr int N = Packet<T>::N, GROUPS = groups_of(WR), THREADS = 32 * WR * GROUPS;
+    constexpr int CTAS = THREADS == 256 ? 2 : 1;
+    constexpr int DEPTH = C * N > 16 ? (sizeof(T) == 2 ? 2 : 1) : kDepth;          // (what fits an SM's shared memory)
+    const bool vec = on_grid(x) && on_grid(dy) && (!dx.data || on_grid(dx)) && on_grid(gamma);
+    const bool full = vec && x.cols == (int64_t)32 * WR * C * N;
+    auto kernel = full  ? norm_backward_resident_kernel<T, P, N, C, WR, GROUPS, DEPTH, CTAS, true>
+                  : vec ? norm_backward_resident_kernel<T, P, N, C, WR, GROUPS, DEPTH, CTAS, false>
+                        : norm_backward_resident_kernel<T, P, 1, C * N, WR, GROUPS, DEPTH, CTAS, false>;
+    float* partial = dgamma || dbeta ? (float*)space : nullptr;
+    const size_t smem = std::max<size_t>(vec ? (size_t)DEPTH * 2 * C * THREADS * 16 : 0, GROUPS > 1 ? 2 * x.cols * sizeof(float) : 0);
+    static std::atomic<unsigned long long> allowed[2];
+    cudaError_t e = allow_shared(kernel, smem, &allowed[full]);
+    if (e != cudaSuccess) return e;
+    e = launch(kernel, dim3((unsigned)b.slices), THREADS, smem, s, 1, (const T*)dy.data, (long long)dy.stride, (const T*)x.data,
+               (long long)x.stride, (const P*)gamma, (T*)dx.data, (long long)dx.stride, (long long)x.rows, (int)x.cols, (float)eps, partial);
+    return e == cudaSuccess && partial ? fold_columns<P>(s, (const float*)partial, b.slices, x.cols, dgamma, dbeta) : e;
+}
+template <typename T, typename P, int C, typename... R>
+cudaError_t backward_resident_of(int warps, R... rest) {
+    switch (warps) {
+        case 1: return backward_resident<T, P, C, 1>(rest...);
+        case 2: return backward_resident<T, P, C, 2>(rest...);
+        case 4: return backward_resident<T, P, C, 4>(rest...);
+        case 8: return backward_resident<T, P, C, 8>(rest...);
+        default: return backward_resident<T, P, C, 16>(rest...);
+    }
 }
 
 template <typename T, typename P>
 cudaError_t backward(cudaStream_t s, const Rows& dy, const Rows& x, const void* gamma, const Rows& dx, void* dgamma, void* dbeta,
                      double eps, void* space) {
     typedef typename AccOf<T>::type A;
-    const BackwardSpace b = backward_space(sizeof(T) == 8 ? DALIB200_F64 : DALIB200_F32, x.rows, x.cols);
+    const BackwardSpace b = backward_space(sizeof(T) == 8 ? DALIB200_F64 : sizeof(T) == 2 ? DALIB200_BF16 : DALIB200_F32, x.rows, x.cols);
+    if constexpr (sizeof(T) < 8) {
+        const Layout l = backward_layout(sizeof(T), x.cols);
+        if (l.warps) {
+            if (l.packets == 2) return backward_resident_of<T, P, 2>(l.warps, s, b, dy, x, gamma, dx, dgamma, dbeta, eps, space);
+            if constexpr (sizeof(T) == 2) {
+                if (l.packets == 1) return backward_resident<T, P, 1, 1>(s, b, dy, x, gamma, dx, dgamma, dbeta, eps, space);
+                return backward_resident<T, P, 4, 16>(s, b, dy, x, gamma, dx, dgamma, dbeta, eps, space);
+            } else {
+                return backward_resident<T, P, 8, 16>(s, b, dy, x, gamma, dx, dgamma, dbeta, eps, space);
+            }
+        }
+    }
     A* stats = (A*)space;
     A* partial = (A*)((char*)space + b.stats);
     const dim3 by_row((unsigned)capped(x.rows, kSms * 64));
@@ -182,9 +719,7 @@ cudaError_t backward(cudaStream_t s, const Rows& dy, const Rows& x, const void* 
         e = launch(column_sums_kernel<T>, dim3((unsigned)((x.cols + kThreads - 1) / kThreads), (unsigned)b.slices), kThreads, 0, s, 1,
                    (const T*)dy.data, (long long)dy.stride, (const T*)x.data, (long long)x.stride, (long long)x.rows,
                    (long long)x.cols, (const A*)stats, partial);
-        if (e == cudaSuccess)
-            e = launch(fold_columns_kernel<A, P>, dim3((unsigned)((x.cols + 31) / 32), 2), kThreads, 0, s, 1, (const A*)partial, b.slices,
-                       (long long)x.cols, (P*)dgamma, (P*)dbeta);
+        if (e == cudaSuccess) e = fold_columns<P>(s, (const A*)partial, b.slices, x.cols, dgamma, dbeta);
     }
     if (e == cudaSuccess && dx.data)
         e = launch(dx_kernel<T, P>, by_row, kThreads, 0, s, 1, (const T*)dy.data, (long long)dy.stride, (const T*)x.data,

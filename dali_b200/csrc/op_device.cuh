@@ -45,6 +45,68 @@ template <typename T> __device__ __forceinline__ void store_packet(T* p, const P
     *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(&v);
 }
 
+// two fp32 values, one instruction
+struct Two { unsigned long long v; };
+__device__ __forceinline__ Two two(float a, float b) {
+    Two r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void parts(Two x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v)); }
+__device__ __forceinline__ Two operator+(Two a, Two b) {
+    Two r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Two operator*(Two a, Two b) {
+    Two r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+    return r;
+}
+__device__ __forceinline__ Two multiply_add(Two a, Two b, Two c) {
+    Two r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return r;
+}
+
+__device__ __forceinline__ Two both(float a) { return two(a, a); }
+__device__ __forceinline__ float total(Two x) {
+    float a, b;
+    parts(x, a, b);
+    return a + b;
+}
+// two bf16 values of one word
+__device__ __forceinline__ Two widen_pair(uint32_t w) { return two(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)); }
+__device__ __forceinline__ uint32_t narrow_pair(Two x) {
+    float a, b;
+    parts(x, a, b);
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(b), "f"(a));
+    return r;
+}
+// a packet of 16 bytes as pairs, and back
+__device__ __forceinline__ void pairs_of(uint4 q, Two (&z)[2], const float*) {
+    z[0] = two(__uint_as_float(q.x), __uint_as_float(q.y));
+    z[1] = two(__uint_as_float(q.z), __uint_as_float(q.w));
+}
+__device__ __forceinline__ void pairs_of(uint4 q, Two (&z)[4], const bf16_s*) {
+    z[0] = widen_pair(q.x);
+    z[1] = widen_pair(q.y);
+    z[2] = widen_pair(q.z);
+    z[3] = widen_pair(q.w);
+}
+__device__ __forceinline__ uint4 packet_of(const Two (&z)[2], const float*) {
+    uint4 q;
+    float a, b, c, d;
+    parts(z[0], a, b);
+    parts(z[1], c, d);
+    q.x = __float_as_uint(a), q.y = __float_as_uint(b), q.z = __float_as_uint(c), q.w = __float_as_uint(d);
+    return q;
+}
+__device__ __forceinline__ uint4 packet_of(const Two (&z)[4], const bf16_s*) {
+    return make_uint4(narrow_pair(z[0]), narrow_pair(z[1]), narrow_pair(z[2]), narrow_pair(z[3]));
+}
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int m = 16; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);

@@ -201,41 +201,7 @@ __device__ __forceinline__ float exp2_of(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
     return r;
 }
-// two fp32 values, one instruction
-struct Two { unsigned long long v; };
-__device__ __forceinline__ Two two(float a, float b) {
-    Two r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(a), "f"(b));
-    return r;
-}
-__device__ __forceinline__ void parts(Two x, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.v)); }
-__device__ __forceinline__ Two operator+(Two a, Two b) {
-    Two r;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-    return r;
-}
-__device__ __forceinline__ Two operator*(Two a, Two b) {
-    Two r;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-    return r;
-}
-__device__ __forceinline__ Two multiply_add(Two a, Two b, Two c) {
-    Two r;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-    return r;
-}
-
-// the packet as pairs of fp32 values, and the largest of its values (NaN counts only if there is nothing else)
-__device__ __forceinline__ void pairs_of(uint4 q, Two (&z)[2], float*) {
-    z[0] = two(__uint_as_float(q.x), __uint_as_float(q.y));
-    z[1] = two(__uint_as_float(q.z), __uint_as_float(q.w));
-}
-__device__ __forceinline__ void pairs_of(uint4 q, Two (&z)[4], bf16_s*) {
-    z[0] = two(__uint_as_float(q.x << 16), __uint_as_float(q.x & 0xffff0000u));
-    z[1] = two(__uint_as_float(q.y << 16), __uint_as_float(q.y & 0xffff0000u));
-    z[2] = two(__uint_as_float(q.z << 16), __uint_as_float(q.z & 0xffff0000u));
-    z[3] = two(__uint_as_float(q.w << 16), __uint_as_float(q.w & 0xffff0000u));
-}
+// the largest value of some packets (NaN counts only if there is nothing else)
 __device__ __forceinline__ uint32_t max_of_pairs(uint32_t a, uint32_t b) {
     uint32_t r;
     asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
