@@ -152,31 +152,44 @@ __global__ void __launch_bounds__(kThreads) fold_columns_kernel(const A* __restr
 // No squares of values far from zero are subtracted from one another, and the backward pass needs no more exchanges with
 // recomputed statistics than it would with saved ones.
 
-// A thread holds C packets of W elements of a row, the row's WR warps side by side (W = 1: rows that are off the 16-byte grid or no
-// whole number of 16-byte packets).  Whole packets come through a ring of DEPTH rows in shared memory that every thread
-// fills and reads for itself (cp.async; no thread waits for another one's copies), so that the loads of the next rows are under way
-// while a row is worked on.
-// FULL: every thread of the row holds all C of them.
-template <int W, int C, int WR, bool FULL>
+// A thread holds C packets of W elements of a row, the row's WR warps side by side.  Packets come through a ring of DEPTH rows in
+// shared memory that every thread fills and reads for itself (cp.async; no thread waits for another one's copies), so that the
+// loads of the next rows are under way while a row is worked on.
+// EDGE: rows that do not lie on the 16-byte grid.  Their packets do; the few elements in front of the first one and behind the last one
+// are one more for each of the row's first threads.  A CTA's rows are a multiple of W apart, so that every thread holds the same
+// columns of all of them.  (W = 1: matrices whose rows do not even lie alike on the grid.)
+enum Rowfit { FULL, WHOLE, EDGE };          // every thread holds C packets; packets are there or not; EDGE
+template <int W, int C, int WR, Rowfit FIT>
 struct Held {
     uint32_t there;          // bit i: the thread's i-th packet is one of the row's
     int first;               // column of the first packet; the others lie 32 WR W columns apart
-    int mine;                // elements that this warp holds
-    __device__ __forceinline__ Held(int t, int cols) : there(0), first(t * W), mine(of_warp(t >> 5, cols)) {
+    int edge;                // column of the thread's edge element, -1: it has none
+    int mine, its;           // elements that this warp holds, and the warp of the row whose sums this lane looks after
+    // `off`: elements by which the rows lie behind the grid
+    __device__ __forceinline__ Held(int t, int cols, int off) : there(0), edge(-1) {
+        const int head = FIT == EDGE && off ? min(W - off, cols) : 0, packets = (cols - head) / W, edges = cols - packets * W;
+        first = head + t * W;
 #pragma unroll
         for (int i = 0; i < C; ++i)
-            if (column(i) < cols) there |= 1u << i;
+            if (t + i * 32 * WR < packets) there |= 1u << i;
+        if (FIT == EDGE && t < edges) edge = t < head ? t : t + packets * W;
+        mine = of_warp(t >> 5, packets, edges);
+        its = of_warp(t & 31 & (WR - 1), packets, edges);
     }
     __device__ __forceinline__ int column(int i) const { return first + i * 32 * WR * W; }
-    __device__ __forceinline__ bool has(int i) const { return FULL || (there >> i & 1); }
-    static __device__ __forceinline__ int of_warp(int w, int cols) {
-        if (FULL) return 32 * C * W;
-        int n = 0;
+    __device__ __forceinline__ bool has(int i) const { return FIT == FULL || (there >> i & 1); }
+    __device__ __forceinline__ bool has_edge() const { return FIT == EDGE && edge >= 0; }
+  private:
+    static __device__ __forceinline__ int of_warp(int w, int packets, int edges) {
+        if (FIT == FULL) return 32 * C * W;
+        int n = FIT == EDGE && w == 0 ? edges : 0;
 #pragma unroll
-        for (int i = 0; i < C; ++i) n += min(max(cols / W - (i * WR + w) * 32, 0), 32) * W;
+        for (int i = 0; i < C; ++i) n += min(max(packets - (i * WR + w) * 32, 0), 32) * W;
         return n;
     }
 };
+template <Rowfit FIT, typename T>
+__device__ __forceinline__ int behind_grid(const T* row) { return FIT == EDGE ? (int)((uintptr_t)row % 16 / sizeof(T)) : 0; }
 
 __device__ __forceinline__ void copy_async(uint4* to, const void* from) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from) : "memory");
@@ -233,16 +246,22 @@ struct Vals {
     }
     template <typename T> __device__ __forceinline__ void read(const T* from) { pairs_of(*reinterpret_cast<const uint4*>(from), p, from); }
     template <typename T> __device__ __forceinline__ void write(T* to) const { *reinterpret_cast<uint4*>(to) = packet_of(p, to); }
-    // weights: W values of any type that lie on the 16-byte grid
-    __device__ __forceinline__ void weights(const float* w) {
+    // weights of W neighbouring columns; they lie on the 16-byte grid, or element by element
+    template <bool GRID, typename P> __device__ __forceinline__ void weights(const P* w) {
+        if constexpr (!GRID) {
 #pragma unroll
-        for (int i = 0; i < W / 4; ++i) {
-            const float4 q = reinterpret_cast<const float4*>(w)[i];
-            p[2 * i] = two(q.x, q.y);
-            p[2 * i + 1] = two(q.z, q.w);
+            for (int e = 0; e < W; e += 2) p[e / 2] = two(widen(w[e]), widen(w[e + 1]));
+        } else if constexpr (sizeof(P) == 2) {
+            read(w);
+        } else {
+#pragma unroll
+            for (int i = 0; i < W / 4; ++i) {
+                const float4 q = reinterpret_cast<const float4*>(w)[i];
+                p[2 * i] = two(q.x, q.y);
+                p[2 * i + 1] = two(q.z, q.w);
+            }
         }
     }
-    __device__ __forceinline__ void weights(const bf16_s* w) { read(w); }
 };
 template <>
 struct Vals<1> {
@@ -259,7 +278,7 @@ struct Vals<1> {
     __device__ __forceinline__ float value(int) const { return f; }
     template <typename T> __device__ __forceinline__ void read(const T* from) { f = widen(*from); }
     template <typename T> __device__ __forceinline__ void write(T* to) const { *to = Narrow<T>::of(f); }
-    template <typename T> __device__ __forceinline__ void weights(const T* w) { f = widen(*w); }
+    template <bool GRID, typename P> __device__ __forceinline__ void weights(const P* w) { f = widen(*w); }
 };
 
 // over WR neighbouring lanes
@@ -287,7 +306,7 @@ __device__ __forceinline__ void row_barrier(int group) {
     else asm volatile("bar.sync 4, %0;" ::"n"(32 * WR) : "memory");
 }
 
-template <typename T, typename P, int W, int C, int WR, int GROUPS, int DEPTH, int CTAS, bool FULL>
+template <typename T, typename P, int W, int C, int WR, int GROUPS, int DEPTH, int CTAS, Rowfit FIT>
 __global__ void __launch_bounds__(32 * WR * GROUPS, CTAS) norm_resident_kernel(const T* x, long long ldx, const P* __restrict__ gamma,
                                                                                const P* __restrict__ beta, T* y, long long ldy,
                                                                                long long rows, int cols, float eps) {
@@ -296,11 +315,12 @@ __global__ void __launch_bounds__(32 * WR * GROUPS, CTAS) norm_resident_kernel(c
     __shared__ float2 sm[2][GROUPS * WR];
     dependent_prologue();
     const int lane = threadIdx.x & 31, group = threadIdx.x / (32 * WR), warp = threadIdx.x / 32 % WR;
-    const Held<W, C, WR, FULL> at(threadIdx.x % (32 * WR), cols);
-    const float per_mine = at.mine ? 1.0f / at.mine : 0.0f, per_col = 1.0f / cols;
-    const float its = Held<W, C, WR, FULL>::of_warp(lane % WR, cols), per_its = its ? 1.0f / its : 0.0f;      // of the warp whose sums this lane looks after
-    const long long step = (long long)gridDim.x * GROUPS;
     long long row = (long long)blockIdx.x * GROUPS + group;
+    const int off = behind_grid<FIT>(x + row * ldx);
+    const Held<W, C, WR, FIT> at(threadIdx.x % (32 * WR), cols, off);
+    const float per_mine = at.mine ? 1.0f / at.mine : 0.0f, per_col = 1.0f / cols;
+    const float its = at.its, per_its = at.its ? 1.0f / at.its : 0.0f;
+    const long long step = (long long)gridDim.x * GROUPS;
     // The weights stay in registers where there are not too many of them: reading them again for every row, 32 bytes for each 16 of
     // a bf16 row, kept L1 85% busy at 40% of the memory's bandwidth (62 us instead of 43 for 16384 x 4096).
     constexpr bool HOLD = C * W <= 16;
@@ -310,8 +330,8 @@ __global__ void __launch_bounds__(32 * WR * GROUPS, CTAS) norm_resident_kernel(c
         for (int i = 0; i < C; ++i) {
             g[i].all(1);
             b[i].all(0);
-            if (gamma && at.has(i)) g[i].weights(gamma + at.column(i));
-            if (beta && at.has(i)) b[i].weights(beta + at.column(i));
+            if (gamma && at.has(i)) g[i].template weights<FIT != EDGE>(gamma + at.column(i));
+            if (beta && at.has(i)) b[i].template weights<FIT != EDGE>(beta + at.column(i));
         }
     }
     const T *from = x + row * ldx, *ahead = from;          // the row, and the next one to be fetched
@@ -330,13 +350,17 @@ __global__ void __launch_bounds__(32 * WR * GROUPS, CTAS) norm_resident_kernel(c
     if (W > 1)
         for (int d = 0; d < DEPTH - 1; ++d) fetch(d);
     int stage = 0, turn = 0;
+    const float edge_g = gamma && at.has_edge() ? widen(gamma[at.edge]) : 1.0f, edge_b = beta && at.has_edge() ? widen(beta[at.edge]) : 0.0f;
+    float edge_next = at.has_edge() && row < rows ? widen(from[at.edge]) : 0.0f;          // a row ahead
     for (; row < rows; row += step, from += step * ldx, to += step * ldy) {
         if (W > 1) {
             fetch(stage ? stage - 1 : DEPTH - 1);
             copies_but<DEPTH - 1>();
         }
         Vals<W> v[C];
-        float sum = 0;
+        const float edge = edge_next;
+        if (at.has_edge() && row + step < rows) edge_next = widen(from[step * ldx + at.edge]);
+        float sum = edge;
 #pragma unroll
         for (int i = 0; i < C; ++i) {
             if (at.has(i)) v[i].read(W > 1 ? (const T*)(ring + (stage * C + i) * THREADS + threadIdx.x) : from + at.column(i));
@@ -354,7 +378,9 @@ __global__ void __launch_bounds__(32 * WR * GROUPS, CTAS) norm_resident_kernel(c
                 d.add(-mean_w);
                 squares.fma(d, d, squares);
             }
-        float q = warp_sum(squares.sum());
+        float q = squares.sum();
+        if (at.has_edge()) q += (edge - mean_w) * (edge - mean_w);
+        q = warp_sum(q);
         float mean = quotient(sum, cols, per_col);
         if (WR > 1) {
             float2* all = sm[turn] + group * WR;
@@ -377,23 +403,24 @@ __global__ void __launch_bounds__(32 * WR * GROUPS, CTAS) norm_resident_kernel(c
                 } else {
                     Vals<W> w;
                     if (gamma) {
-                        w.weights(gamma + at.column(i));
+                        w.template weights<FIT != EDGE>(gamma + at.column(i));
                         v[i].mul(w);
                     }
                     if (beta) {
-                        w.weights(beta + at.column(i));
+                        w.template weights<FIT != EDGE>(beta + at.column(i));
                         v[i].add(w);
                     }
                 }
                 v[i].write(to + at.column(i));
             }
+        if (at.has_edge()) to[at.edge] = Narrow<T>::of((edge - mean) * r * edge_g + edge_b);
         stage = stage + 1 == DEPTH ? 0 : stage + 1;
     }
 }
 
 // Every CTA takes rows gridDim.x * GROUPS apart, sums dy h and dy of its columns in registers and leaves them, its groups added in
 // their order, in partial[CTA][0 / 1].
-template <typename T, typename P, int W, int C, int WR, int GROUPS, int DEPTH, int CTAS, bool FULL>
+template <typename T, typename P, int W, int C, int WR, int GROUPS, int DEPTH, int CTAS, Rowfit FIT>
 __global__ void __launch_bounds__(32 * WR * GROUPS, CTAS)
     norm_backward_resident_kernel(const T* dy, long long lddy, const T* x, long long ldx, const P* __restrict__ gamma, T* dx, long long lddx,
                                   long long rows, int cols, float eps, float* __restrict__ partial) {
@@ -402,11 +429,12 @@ __global__ void __launch_bounds__(32 * WR * GROUPS, CTAS)
     __shared__ float4 sm[2][GROUPS * WR];
     dependent_prologue();
     const int lane = threadIdx.x & 31, group = threadIdx.x / (32 * WR), warp = threadIdx.x / 32 % WR;
-    const Held<W, C, WR, FULL> at(threadIdx.x % (32 * WR), cols);
-    const float per_mine = at.mine ? 1.0f / at.mine : 0.0f, per_col = 1.0f / cols;
-    const float its = Held<W, C, WR, FULL>::of_warp(lane % WR, cols), per_its = its ? 1.0f / its : 0.0f;      // of the warp whose sums this lane looks after
-    const long long step = (long long)gridDim.x * GROUPS;
     long long row = (long long)blockIdx.x * GROUPS + group;
+    const int off = behind_grid<FIT>(x + row * ldx);
+    const Held<W, C, WR, FIT> at(threadIdx.x % (32 * WR), cols, off);
+    const float per_mine = at.mine ? 1.0f / at.mine : 0.0f, per_col = 1.0f / cols;
+    const float its = at.its, per_its = at.its ? 1.0f / at.its : 0.0f;
+    const long long step = (long long)gridDim.x * GROUPS;
     // Up to 16 values a thread, the row and its weights stay in registers across the exchange; above, they are read again behind it
     // (the row from the ring, the weights from L1), and the sums of the columns have the registers.
     constexpr bool HOLD = C * W <= 16;
@@ -414,7 +442,7 @@ __global__ void __launch_bounds__(32 * WR * GROUPS, CTAS)
     Vals<W> g[H], dg[C], db[C];
     auto weigh = [&](int i) {
         g[HOLD ? i : 0].all(1);
-        if (gamma && at.has(i)) g[HOLD ? i : 0].weights(gamma + at.column(i));
+        if (gamma && at.has(i)) g[HOLD ? i : 0].template weights<FIT != EDGE>(gamma + at.column(i));
     };
 #pragma unroll
     for (int i = 0; i < C; ++i) {
@@ -443,15 +471,30 @@ __global__ void __launch_bounds__(32 * WR * GROUPS, CTAS)
     if (W > 1)
         for (int d = 0; d < DEPTH - 1; ++d) fetch(d);
     int stage = 0, turn = 0;
+    const float edge_g = gamma && at.has_edge() ? widen(gamma[at.edge]) : 1.0f;
+    float edge_dg = 0, edge_db = 0, edge_x_next = 0, edge_dy_next = 0;          // (the next row's: a row ahead)
+    if (at.has_edge() && row < rows) {
+        edge_x_next = widen(from_x[at.edge]);
+        edge_dy_next = widen(from_dy[at.edge]);
+    }
     for (; row < rows; row += step, from_x += step * ldx, from_dy += step * lddy, to_dx += step * lddx) {
         if (W > 1) {
             fetch(stage ? stage - 1 : DEPTH - 1);
             copies_but<DEPTH - 1>();
         }
         Vals<W> v[H], u[H];
-        float sum = 0;
-        auto read_x = [&](int i) { v[HOLD ? i : 0].read(W > 1 ? (const T*)slot(stage, 0, i) : from_x + at.column(i)); };
-        auto read_dy = [&](int i) { u[HOLD ? i : 0].read(W > 1 ? (const T*)slot(stage, 1, i) : from_dy + at.column(i)); };
+        float edge_x = edge_x_next, edge_dy = edge_dy_next;
+        if (at.has_edge() && row + step < rows) {
+            edge_x_next = widen(from_x[step * ldx + at.edge]);
+            edge_dy_next = widen(from_dy[step * lddy + at.edge]);
+        }
+        float sum = edge_x;
+        auto read_x = [&](int i) {
+            v[HOLD ? i : 0].read(W > 1 ? (const T*)slot(stage, 0, i) : from_x + at.column(i));
+        };
+        auto read_dy = [&](int i) {
+            u[HOLD ? i : 0].read(W > 1 ? (const T*)slot(stage, 1, i) : from_dy + at.column(i));
+        };
 #pragma unroll
         for (int i = 0; i < C; ++i)
             if (at.has(i)) {
@@ -481,7 +524,16 @@ __global__ void __launch_bounds__(32 * WR * GROUPS, CTAS)
                 sa.add(ae);
                 sc.fma(ae, d, sc);
             }
-        float q = warp_sum(sq.sum()), a = warp_sum(sa.sum()), c = warp_sum(sc.sum());
+        float q = sq.sum(), a = sa.sum(), c = sc.sum();
+        if (at.has_edge()) {
+            const float d = edge_x - mean_w, ae = edge_dy * edge_g;
+            q += d * d;
+            a += ae;
+            c += ae * d;
+        }
+        q = warp_sum(q);
+        a = warp_sum(a);
+        c = warp_sum(c);
         float mean = quotient(sum, cols, per_col);
         if (WR > 1) {
             float4* all = sm[turn] + group * WR;
@@ -514,6 +566,13 @@ __global__ void __launch_bounds__(32 * WR * GROUPS, CTAS)
                 u[k].fma(v[k], c2, u[k]);
                 if (dx) u[k].write(to_dx + at.column(i));
             }
+        if (at.has_edge()) {
+            edge_x -= mean;
+            edge_db += edge_dy;
+            edge_dy *= r;
+            edge_dg += edge_dy * edge_x;
+            if (dx) to_dx[at.edge] = Narrow<T>::of(edge_dy * edge_g + c1 + edge_x * c2);
+        }
         stage = stage + 1 == DEPTH ? 0 : stage + 1;
     }
     if (!partial) return;
@@ -533,6 +592,11 @@ __global__ void __launch_bounds__(32 * WR * GROUPS, CTAS)
                     }
                 }
         }
+        if (group == k && at.has_edge()) {
+            float *pg = (GROUPS == 1 ? to : columns) + at.edge, *pb = pg + cols;
+            *pg = k ? *pg + edge_dg : edge_dg;
+            *pb = k ? *pb + edge_db : edge_db;
+        }
         if (GROUPS > 1) __syncthreads();
     }
     if (GROUPS > 1)
@@ -549,7 +613,7 @@ Layout forward_layout(int size, int64_t cols) {
     const int64_t packets = (cols + 16 / size - 1) / (16 / size);
     Layout l = {size == 2 ? 2 : 4, 1};
     if (packets <= 32ll * l.packets / 2) l.packets /= 2;
-    else if (size == 2 && packets > 32 * 8 * 2) l.packets = 4;
+    else if (size == 2 && packets > 32 * 32 * 2) l.packets = 4;
     while (l.warps <= 32 && 32ll * l.packets * l.warps < packets) l.warps *= 2;
     if (l.warps > 32) l.warps = 0;
     return l;
@@ -559,14 +623,19 @@ Layout forward_layout(int size, int64_t cols) {
 Layout backward_layout(int size, int64_t cols) {
     const int64_t packets = (cols + 16 / size - 1) / (16 / size);
     Layout l = {size == 2 && packets <= 32 ? 1 : 2, 1};
-    while (l.warps <= 16 && 32ll * l.packets * l.warps < packets) l.warps *= 2;
-    if (l.warps > 16) l = {size == 2 ? 4 : 8, 32ll * 16 * (size == 2 ? 4 : 8) < packets ? 0 : 16};
+    const int most = size == 2 ? 16 : 32;
+    while (l.warps <= most && 32ll * l.packets * l.warps < packets) l.warps *= 2;
+    if (l.warps > most) l = {size == 2 ? 4 : 8, 32ll * 16 * (size == 2 ? 4 : 8) < packets ? 0 : 16};
     return l;
 }
-bool on_grid(const void* p) { return (uintptr_t)p % 16 == 0; }
-bool on_grid(const Rows& m) {
-    return (uintptr_t)m.data % 16 == 0 && m.cols % (16 / m.size) == 0 && (m.rows < 2 || m.stride % (16 / m.size) == 0);
+// Do the rows of two matrices lie alike on the 16-byte grid?
+bool alike(const Rows& a, const Rows& b) {
+    return ((uintptr_t)a.data - (uintptr_t)b.data) % 16 == 0 && (a.rows < 2 || (a.stride - b.stride) * a.size % 16 == 0);
 }
+bool on_grid(const void* p) { return (uintptr_t)p % 16 == 0; }
+bool on_grid(const Rows& m) { return (uintptr_t)m.data % 16 == 0 && (m.rows < 2 || m.stride * m.size % 16 == 0); }
+// at most that many CTAs, a multiple of 8, so that the rows of one lie alike on the grid
+long long capped_alike(long long want, long long most) { return want <= most ? std::max(want, 1ll) : most / 8 * 8; }
 
 long long capped(long long want, long long most) { return std::max<long long>(1, std::min(want, most)); }
 
@@ -578,7 +647,7 @@ long long column_slices(long long rows, long long cols) {
 // A CTA that holds 16 values a thread in 256 threads takes half of an SM's registers.
 long long backward_ctas(const Layout& l, int64_t rows) {
     const int groups = groups_of(l.warps);
-    return capped((rows + groups - 1) / groups, kSms * (l.warps > 8 ? 1 : 2));
+    return capped_alike((rows + groups - 1) / groups, kSms * (l.warps > 8 ? 1 : 2));
 }
 
 struct BackwardSpace { size_t stats, partial, total; long long slices; };
@@ -615,17 +684,18 @@ template <typename T, typename P, int C, int WR>
 cudaError_t forward_resident(cudaStream_t s, const Rows& x, const void* gamma, const void* beta, const Rows& y, double eps) {
     constexpr int N = Packet<T>::N, GROUPS = groups_of(WR), THREADS = 32 * WR * GROUPS;
     constexpr int CTAS = THREADS == 256 ? (C * N > 16 ? 2 : C * N > 8 ? 3 : 4) : THREADS == 512 ? (C * N > 8 ? 1 : 2) : 1;
-    const bool vec = on_grid(x) && on_grid(y) && on_grid(gamma) && on_grid(beta);
-    const bool full = vec && x.cols == (int64_t)32 * WR * C * N;
-    auto kernel = full  ? norm_resident_kernel<T, P, N, C, WR, GROUPS, kDepth, CTAS, true>
-                  : vec ? norm_resident_kernel<T, P, N, C, WR, GROUPS, kDepth, CTAS, false>
-                        : norm_resident_kernel<T, P, 1, C * N, WR, GROUPS, kDepth, CTAS, false>;
+    const bool vec = alike(x, y);
+    const bool whole = vec && on_grid(x) && x.cols % N == 0 && on_grid(gamma) && on_grid(beta), full = whole && x.cols == (int64_t)32 * WR * C * N;
+    auto kernel = full    ? norm_resident_kernel<T, P, N, C, WR, GROUPS, kDepth, CTAS, FULL>
+                  : whole ? norm_resident_kernel<T, P, N, C, WR, GROUPS, kDepth, CTAS, WHOLE>
+                  : vec   ? norm_resident_kernel<T, P, N, C, WR, GROUPS, kDepth, CTAS, EDGE>
+                          : norm_resident_kernel<T, P, 1, C * N, WR, GROUPS, kDepth, CTAS, WHOLE>;
     const size_t smem = vec ? (size_t)kDepth * C * THREADS * 16 : 0;
-    static std::atomic<unsigned long long> allowed[2];
-    const cudaError_t e = allow_shared(kernel, smem, &allowed[full]);
+    static std::atomic<unsigned long long> allowed[3];
+    const cudaError_t e = allow_shared(kernel, smem, &allowed[full ? 0 : whole ? 1 : 2]);
     if (e != cudaSuccess) return e;
     const long long ctas = (x.rows + GROUPS - 1) / GROUPS;
-    return launch(kernel, dim3((unsigned)capped(ctas, kSms * (vec ? CTAS : 32))), THREADS, smem, s, 1,
+    return launch(kernel, dim3((unsigned)capped_alike(ctas, kSms * (vec ? CTAS : 32))), THREADS, smem, s, 1,
                   (const T*)x.data, (long long)x.stride, (const P*)gamma, (const P*)beta, (T*)y.data, (long long)y.stride,
                   (long long)x.rows, (int)x.cols, (float)eps);
 }
@@ -668,15 +738,16 @@ cudaError_t backward_resident(cudaStream_t s, const BackwardSpace& b, const Rows
     constexpr int N = Packet<T>::N, GROUPS = groups_of(WR), THREADS = 32 * WR * GROUPS;
     constexpr int CTAS = THREADS == 256 ? 2 : 1;
     constexpr int DEPTH = C * N > 16 ? (sizeof(T) == 2 ? 2 : 1) : kDepth;          // (what fits an SM's shared memory)
-    const bool vec = on_grid(x) && on_grid(dy) && (!dx.data || on_grid(dx)) && on_grid(gamma);
-    const bool full = vec && x.cols == (int64_t)32 * WR * C * N;
-    auto kernel = full  ? norm_backward_resident_kernel<T, P, N, C, WR, GROUPS, DEPTH, CTAS, true>
-                  : vec ? norm_backward_resident_kernel<T, P, N, C, WR, GROUPS, DEPTH, CTAS, false>
-                        : norm_backward_resident_kernel<T, P, 1, C * N, WR, GROUPS, DEPTH, CTAS, false>;
+    const bool vec = alike(x, dy) && (!dx.data || alike(x, dx));
+    const bool whole = vec && on_grid(x) && x.cols % N == 0 && on_grid(gamma), full = whole && x.cols == (int64_t)32 * WR * C * N;
+    auto kernel = full    ? norm_backward_resident_kernel<T, P, N, C, WR, GROUPS, DEPTH, CTAS, FULL>
+                  : whole ? norm_backward_resident_kernel<T, P, N, C, WR, GROUPS, DEPTH, CTAS, WHOLE>
+                  : vec   ? norm_backward_resident_kernel<T, P, N, C, WR, GROUPS, DEPTH, CTAS, EDGE>
+                          : norm_backward_resident_kernel<T, P, 1, C * N, WR, GROUPS, DEPTH, CTAS, WHOLE>;
     float* partial = dgamma || dbeta ? (float*)space : nullptr;
     const size_t smem = std::max<size_t>(vec ? (size_t)DEPTH * 2 * C * THREADS * 16 : 0, GROUPS > 1 ? 2 * x.cols * sizeof(float) : 0);
-    static std::atomic<unsigned long long> allowed[2];
-    cudaError_t e = allow_shared(kernel, smem, &allowed[full]);
+    static std::atomic<unsigned long long> allowed[3];
+    cudaError_t e = allow_shared(kernel, smem, &allowed[full ? 0 : whole ? 1 : 2]);
     if (e != cudaSuccess) return e;
     e = launch(kernel, dim3((unsigned)b.slices), THREADS, smem, s, 1, (const T*)dy.data, (long long)dy.stride, (const T*)x.data,
                (long long)x.stride, (const P*)gamma, (T*)dx.data, (long long)dx.stride, (long long)x.rows, (int)x.cols, (float)eps, partial);
@@ -689,7 +760,10 @@ cudaError_t backward_resident_of(int warps, R... rest) {
         case 2: return backward_resident<T, P, C, 2>(rest...);
         case 4: return backward_resident<T, P, C, 4>(rest...);
         case 8: return backward_resident<T, P, C, 8>(rest...);
-        default: return backward_resident<T, P, C, 16>(rest...);
+        case 16: return backward_resident<T, P, C, 16>(rest...);
+        default:
+            if constexpr (sizeof(T) == 4) return backward_resident<T, P, C, 32>(rest...);
+            return cudaErrorInvalidValue;          // (no layout of 16-bit rows has more than 16 warps)
     }
 }
 
