@@ -44,14 +44,34 @@ __device__ __forceinline__ int tensor_of(const List& l, long long chunk) {
     return lo;
 }
 
+constexpr int kBatch = 4;                    // packets a thread has under way
+
+__device__ __forceinline__ double square(double s, float v) { const double d = (double)v; return fma(d, d, s); }
+__device__ __forceinline__ double square(double s, double v) { return fma(v, v, s); }
+
 template <typename T>
 __device__ __forceinline__ double sum_chunk(const T* x, int n) {
-    double s = 0;
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-        const double v = (double)widen(x[i]);
-        s += v * v;
+    constexpr int N = Packet<T>::N;
+    const int head = min(n, (int)((16 - (uintptr_t)x % 16) % 16 / sizeof(T))), packets = (n - head) / N, edges = n - packets * N;
+    const T* body = x + head;
+    double s = 0, s2 = 0;
+    if ((int)threadIdx.x < edges) s = square(s, widen(x[(int)threadIdx.x < head ? threadIdx.x : threadIdx.x + packets * N]));
+    for (int p = threadIdx.x; p < packets; p += kBatch * kThreads) {
+        Packet<T> q[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+            if (p + i * kThreads < packets) q[i] = load_packet(body + (p + i * kThreads) * N);
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+            if (p + i * kThreads < packets) {
+#pragma unroll
+                for (int e = 0; e < N; e += 2) {
+                    s = square(s, widen(q[i].v[e]));
+                    s2 = square(s2, widen(q[i].v[e + 1]));
+                }
+            }
     }
-    return s;
+    return s + s2;
 }
 
 __global__ void __launch_bounds__(kThreads) squares_kernel(const __grid_constant__ List l, double* __restrict__ partial) {
@@ -94,7 +114,29 @@ __global__ void __launch_bounds__(kThreads) total_kernel(const double* __restric
 
 template <typename T, typename F>
 __device__ __forceinline__ void scale_chunk(const T* x, T* y, int n, F f) {
-    for (int i = threadIdx.x; i < n; i += kThreads) y[i] = Narrow<T>::of(widen(x[i]) * f);
+    constexpr int N = Packet<T>::N;
+    if (((uintptr_t)x - (uintptr_t)y) % 16 != 0) {          // no packet of one is a packet of the other
+        for (int i = threadIdx.x; i < n; i += kThreads) y[i] = Narrow<T>::of(widen(x[i]) * f);
+        return;
+    }
+    const int head = min(n, (int)((16 - (uintptr_t)x % 16) % 16 / sizeof(T))), packets = (n - head) / N, edges = n - packets * N;
+    if ((int)threadIdx.x < edges) {
+        const int i = (int)threadIdx.x < head ? threadIdx.x : threadIdx.x + packets * N;
+        y[i] = Narrow<T>::of(widen(x[i]) * f);
+    }
+    for (int p = threadIdx.x; p < packets; p += kBatch * kThreads) {
+        Packet<T> q[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+            if (p + i * kThreads < packets) q[i] = load_packet(x + head + (p + i * kThreads) * N);
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+            if (p + i * kThreads < packets) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) q[i].v[e] = Narrow<T>::of(widen(q[i].v[e]) * f);
+                store_packet(y + head + (p + i * kThreads) * N, q[i]);
+            }
+    }
 }
 
 __global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__ List l, const double* __restrict__ partial, int n_partial,
@@ -106,7 +148,8 @@ __global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__
     const double n = sqrt(sum);
     const bool down = n > max_norm && n <= DBL_MAX;
     const double f = down ? max_norm / n : 1.0;
-    for (long long c = blockIdx.x; c < l.first[l.n]; c += gridDim.x) {
+    // from the end of the list: what has been read last for the sum is still in L2
+    for (long long c = l.first[l.n] - 1 - blockIdx.x; c >= 0; c -= gridDim.x) {
         const int t = tensor_of(l, c);
         if (!down && l.in[t] == l.out[t]) continue;
         const long long at = (c - l.first[t]) * kChunk;
@@ -187,7 +230,7 @@ cudaError_t queue_squares(cudaStream_t s, const Tensors& t, double* partial) {
 
 cudaError_t queue_scale(cudaStream_t s, const Tensors& t, const double* partial, int n_partial, double max_norm, void* norm, int norm_f64) {
     cudaError_t e = cudaSuccess;
-    for (size_t i = 0; i < t.lists.size() && e == cudaSuccess; ++i)
+    for (size_t i = t.lists.size(); i-- > 0 && e == cudaSuccess;)
         e = launch(scale_kernel, dim3(t.ctas(t.lists[i])), kThreads, 0, s, 1, t.lists[i], partial, n_partial, max_norm,
                    i == 0 ? norm : nullptr, norm_f64);
     return e;

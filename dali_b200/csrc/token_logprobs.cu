@@ -531,14 +531,16 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const T* __restrict_
     if (!started) cluster_wait();
 }
 
+// ---------------------------------------------------------------------------------------------- gradient
+// f64 rows, and rows of logits and gradients that do not lie alike on the 16-byte grid: a CTA per row, element by element.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) logprobs_backward_kernel(const T* logits, long long ld, long long rows, int vocab,
-                                                                     const int* __restrict__ tokens,
-                                                                     const typename AccOf<T>::type* __restrict__ lse,
-                                                                     const typename AccOf<T>::type* __restrict__ entropy,
-                                                                     const typename AccOf<T>::type* __restrict__ dlogprob,
-                                                                     const typename AccOf<T>::type* __restrict__ dentropy, T* dlogits,
-                                                                     long long ldd) {
+__global__ void __launch_bounds__(kThreads) logprobs_backward_rows_kernel(const T* logits, long long ld, long long rows, int vocab,
+                                                                          const int* __restrict__ tokens,
+                                                                          const typename AccOf<T>::type* __restrict__ lse,
+                                                                          const typename AccOf<T>::type* __restrict__ entropy,
+                                                                          const typename AccOf<T>::type* __restrict__ dlogprob,
+                                                                          const typename AccOf<T>::type* __restrict__ dentropy, T* dlogits,
+                                                                          long long ldd) {
     typedef typename AccOf<T>::type A;
     dependent_prologue();
     for (long long row = blockIdx.x; row < rows; row += gridDim.x) {
@@ -558,6 +560,69 @@ __global__ void __launch_bounds__(kThreads) logprobs_backward_kernel(const T* lo
                 if (j == t) d += g;
             }
             out[j] = Narrow<T>::of(d);
+        }
+    }
+}
+
+// Everything else streams: a CTA takes kBatch packets a thread of one row, all loaded before the first is worked on, and p is
+// exp2 of t = (z - lse) log2 e.  With dentropy:  dz = -p (g + w (log p + H)) = -p (a + b t),  a = g + w H, b = w / log2 e.
+template <typename T, bool ENTROPY>
+__global__ void __launch_bounds__(kThreads) logprobs_backward_kernel(const T* logits, long long ld, long long pieces, int per_row, int vocab,
+                                                                     const int* __restrict__ tokens, const float* __restrict__ lse,
+                                                                     const float* __restrict__ entropy, const float* __restrict__ dlogprob,
+                                                                     const float* __restrict__ dentropy, T* dlogits, long long ldd) {
+    constexpr int N = Packet<T>::N;
+    dependent_prologue();
+    for (long long piece = blockIdx.x; piece < pieces; piece += gridDim.x) {
+        const long long r = piece / per_row;
+        const int part = (int)(piece - r * per_row);
+        const RowSplit<T> row(logits + r * ld, vocab);
+        T* out = dlogits + r * ldd;
+        const int t = dlogprob ? tokens[r] : -1;
+        const float g = t < 0 ? 0.0f : t >= vocab ? nan_of(0.0f) : dlogprob[r], l = lse[r];
+        const float w = ENTROPY ? dentropy[r] : 0.0f, h = ENTROPY ? entropy[r] : 0.0f;
+        const bool nothing = (g == 0 && w == 0) || l == -infinity_of(0.0f);
+        const float a = -(g + w * h), b = -w * kLn2;
+        const int begin = part * kBatch * kThreads + threadIdx.x;
+        if (nothing) {          // 0 whatever the logits hold: they are not read
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i)
+                if (begin + i * kThreads < row.packets) *reinterpret_cast<uint4*>(out + row.first_of(begin + i * kThreads)) = make_uint4(0, 0, 0, 0);
+            if (part == 0 && (int)threadIdx.x < row.head + row.tail) out[row.edge(threadIdx.x)] = Narrow<T>::of(0.0f);
+            continue;
+        }
+        uint4 q[kBatch];
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i)
+            if (begin + i * kThreads < row.packets) q[i] = row.packet(begin + i * kThreads);
+#pragma unroll
+        for (int i = 0; i < kBatch; ++i) {
+            const int p = begin + i * kThreads;
+            if (p >= row.packets) break;
+            Two z[N / 2];
+            pairs_of(q[i], z, (const T*)nullptr);
+#pragma unroll
+            for (int e = 0; e < N / 2; ++e) {
+                float t0, t1;
+                parts((z[e] + both(-l)) * both(kLog2e), t0, t1);
+                if (ENTROPY) {
+                    t0 = max_nan(t0, kFloor);
+                    t1 = max_nan(t1, kFloor);
+                }
+                const Two prob = two(exp2_of(t0), exp2_of(t1));
+                z[e] = prob * (ENTROPY ? multiply_add(two(t0, t1), both(b), both(a)) : both(a));
+            }
+            const int j = t - row.first_of(p);
+            if (j >= 0 && j < N) {
+#pragma unroll
+                for (int e = 0; e < N / 2; ++e) z[e] = z[e] + two(j == 2 * e ? g : 0.0f, j == 2 * e + 1 ? g : 0.0f);
+            }
+            *reinterpret_cast<uint4*>(out + row.first_of(p)) = packet_of(z, (const T*)nullptr);
+        }
+        if (part == 0 && (int)threadIdx.x < row.head + row.tail) {
+            const int j = row.edge(threadIdx.x);
+            const float t0 = max_nan((widen(row.z[j]) - l) * kLog2e, kFloor);
+            out[j] = Narrow<T>::of(exp2_of(t0) * (t0 * b + a) + (j == t ? g : 0.0f));
         }
     }
 }
@@ -599,7 +664,17 @@ template <typename T>
 cudaError_t backward(cudaStream_t s, const Rows& z, const int* tokens, const void* lse, const void* entropy, const void* dlogprob,
                      const void* dentropy, const Rows& dz) {
     typedef typename AccOf<T>::type A;
-    return launch(logprobs_backward_kernel<T>, dim3((unsigned)capped(z.rows, kSms * 64)), kThreads, 0, s, 1, (const T*)z.data,
+    const bool alike = ((uintptr_t)z.data - (uintptr_t)dz.data) % 16 == 0 && (z.rows < 2 || (z.stride - dz.stride) * z.size % 16 == 0);
+    if constexpr (sizeof(T) < 8) {
+        if (alike) {
+            const long long packets = z.cols / Packet<T>::N, per_row = std::max<long long>(1, (packets + kBatch * kThreads - 1) / (kBatch * kThreads));
+            const long long pieces = z.rows * per_row;
+            return launch(dentropy ? logprobs_backward_kernel<T, true> : logprobs_backward_kernel<T, false>, dim3((unsigned)capped(pieces, 1 << 30)),
+                          kThreads, 0, s, 1, (const T*)z.data, (long long)z.stride, pieces, (int)per_row, (int)z.cols, tokens, (const float*)lse,
+                          (const float*)entropy, (const float*)dlogprob, (const float*)dentropy, (T*)dz.data, (long long)dz.stride);
+        }
+    }
+    return launch(logprobs_backward_rows_kernel<T>, dim3((unsigned)capped(z.rows, kSms * 64)), kThreads, 0, s, 1, (const T*)z.data,
                   (long long)z.stride, (long long)z.rows, (int)z.cols, tokens, (const A*)lse, (const A*)entropy, (const A*)dlogprob,
                   (const A*)dentropy, (T*)dz.data, (long long)dz.stride);
 }
