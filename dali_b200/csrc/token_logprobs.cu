@@ -182,15 +182,17 @@ __global__ void __launch_bounds__(kThreads) logprobs_rows_kernel(const T* __rest
 }
 
 // ---------------------------------------------------------------------------------------------- f32 and bf16 rows
-// A cluster of S CTAs shares a row, each a contiguous slice of its 16-byte packets; a thread takes every kThreads-th packet of
-// its CTA's slice, kBatch of them at a time, and keeps (m, s, u) in units of log 2: t = (z - m) log2 e, s = sum 2^t,
+// A team of one warp (short rows), of the CTA's eight, or of a cluster of CTAs shares a row, each CTA a contiguous slice of its
+// 16-byte packets; a thread takes every TEAM-th packet of its slice, kBatch of them at a time, and keeps (m, s, u) in units of log 2: t = (z - m) log2 e, s = sum 2^t,
 // u = sum t 2^t.  (z - m is formed before it is scaled: a row of the type's lowest value is uniform, not -infinity.)
 //
-// The alternatives cost no work in that pass.  The entries of one thread are a GROUP; a thread remembers in which batch its
-// maximum was raised last.  At least `top` entries are >= the top-th largest group maximum tau (by value, then index: a total order),
-// and every entry >= tau lies in one of those `top` groups: only they are read again (from L2, 1 / 256 of a CTA's slice each), and
-// what is >= tau in them, hardly more than `top` entries, is sorted.  Lists of 32 keys, one a lane, are sorted and merged
-// bitonically.
+// The alternatives cost no work in that pass.  A thread remembers its largest entry; the largest of a few neighbouring threads is
+// their GROUP's.  At least `top` entries are >= the top-th largest group maximum tau, and every entry >= tau is one of a thread whose own
+// maximum is >= tau: only those threads' entries, hardly more than `top` threads', are read again (from L2), and what is >= tau
+// among them, hardly more than `top` entries, goes to a pool and is put in order by counting for each how many are larger.
+// Where many entries equal tau the pool overflows: then tau is told apart by index too (a larger value, or the same
+// at a lower index; no two entries are the same), for which every thread looks its maximum's place up.  Should even so the
+// pool be too small (all of a few threads' entries larger than every other's), entries are sorted 32 at a time and merged.
 constexpr int kBatch = 4;
 constexpr int kWarps = kThreads / 32;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -236,11 +238,18 @@ struct Running2 {
         s = c * s;
         m = to;
     }
-    __device__ __forceinline__ void merge(Running2 o) {
-        if (o.m > m) raise(o.m);
-        else if (m > o.m) o.raise(m);
-        s += o.s;
-        u += o.u;
+    // the team's: raised to the largest m first, so that sums are left to add; over LANES neighbouring lanes
+    template <int LANES>
+    __device__ __forceinline__ void over_lanes() {
+        float high = m;
+#pragma unroll
+        for (int k = LANES / 2; k > 0; k >>= 1) high = fmaxf(high, __shfl_xor_sync(0xffffffffu, high, k));
+        raise(high);
+#pragma unroll
+        for (int k = LANES / 2; k > 0; k >>= 1) {
+            s += __shfl_xor_sync(0xffffffffu, s, k);
+            u += __shfl_xor_sync(0xffffffffu, u, k);
+        }
     }
 };
 
@@ -269,13 +278,20 @@ __device__ __forceinline__ Key join(Key a, const Key* b, int lane) {
     const Key o = b[31 - lane];
     return merge_down(a > o ? a : o, lane);
 }
-// The 32 largest keys of `n` (a power of two <= 2 * kWarps) descending lists in shared memory, left in list 0.
+// the threads of a team meet
+template <int WR>
+__device__ __forceinline__ void team_barrier() {
+    if (WR == 1) __syncwarp();
+    else __syncthreads();
+}
+// The 32 largest keys of `n` (a power of two <= 2 * WR) descending lists in shared memory, left in list 0.
+template <int WR>
 __device__ __forceinline__ void join_lists(Key (*lists)[32], int n) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    __syncthreads();
+    const int lane = threadIdx.x & 31, warp = (threadIdx.x >> 5) % WR;
+    team_barrier<WR>();
     for (int half = n >> 1; half > 0; half >>= 1) {
         if (warp < half) lists[warp][lane] = join(lists[warp][lane], lists[warp + half], lane);
-        __syncthreads();
+        team_barrier<WR>();
     }
 }
 
@@ -315,102 +331,223 @@ struct RowSplit {
     __device__ __forceinline__ int edge(int i) const { return i < head ? i : i + packets * N; }
 };
 
+// the e-th entry of a packet
 template <typename T>
-__device__ __forceinline__ float entry(uint4 q, int e);
-template <> __device__ __forceinline__ float entry<float>(uint4 q, int e) { return __uint_as_float(e == 0 ? q.x : e == 1 ? q.y : e == 2 ? q.z : q.w); }
-template <> __device__ __forceinline__ float entry<bf16_s>(uint4 q, int e) {
-    const uint32_t w = (e >> 1) == 0 ? q.x : (e >> 1) == 1 ? q.y : (e >> 1) == 2 ? q.z : q.w;
-    return __uint_as_float(e & 1 ? w & 0xffff0000u : w << 16);
+__device__ __forceinline__ float entry(uint4 q, int e) {
+    const int w = sizeof(T) == 4 ? e : e >> 1;
+    const uint32_t word = w & 2 ? (w & 1 ? q.w : q.z) : (w & 1 ? q.y : q.x);
+    return __uint_as_float(sizeof(T) == 4 ? word : e & 1 ? word & 0xffff0000u : word << 16);
+}
+// one bit for each entry of a packet that is >= z
+template <typename T>
+__device__ __forceinline__ uint32_t reaching(uint4 q, float z) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+    uint32_t bits = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (sizeof(T) == 4) {
+            if (__uint_as_float(w[i]) >= z) bits |= 1u << i;
+        } else {
+            if (__uint_as_float(w[i] << 16) >= z) bits |= 1u << 2 * i;
+            if (__uint_as_float(w[i] & 0xffff0000u) >= z) bits |= 2u << 2 * i;
+        }
+    }
+    return bits;
 }
 
-// The `top` largest entries of the CTA's packets [begin, end) (and, in the first CTA, of the row's edges) as a descending list in lists[0].
-// best_batch: the thread's batch whose maximum raised its own last, -1: none did (nothing but -infinity and NaN).
-template <typename T>
-__device__ __forceinline__ void top_of_slice(const RowSplit<T>& row, int begin, int end, bool edges, int top, int best_batch, Key (*lists)[32],
-                                             Key (*pending)[64]) {
-    constexpr int N = Packet<T>::N;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+// `count` distinct keys in shared memory (a zero behind an odd count) -> the 32 largest in descending order in sorted[] (which held
+// zeros).  SPLIT neighbouring threads count for one key.
+template <int TEAM, int SPLIT>
+__device__ __forceinline__ void order_by(const Key* keys, int count, Key* sorted) {
+    const int t = threadIdx.x % TEAM, part = t % SPLIT;
+    for (int i0 = 0; i0 < count; i0 += TEAM / SPLIT) {
+        const int i = i0 + t / SPLIT;
+        const Key mine = i < count ? keys[i] : 0;
+        int larger = 0;
+#pragma unroll 4
+        for (int j = 2 * part; j < count; j += 2 * SPLIT) {
+            const ulonglong2 o = *reinterpret_cast<const ulonglong2*>(keys + j);
+            larger += (o.x > mine) + (o.y > mine);
+        }
+#pragma unroll
+        for (int m = 1; m < SPLIT; m <<= 1) larger += __shfl_xor_sync(0xffffffffu, larger, m);
+        if (part == 0 && mine != 0 && larger < 32) sorted[larger] = mine;
+    }
+}
+template <int TEAM>
+__device__ __forceinline__ void order(const Key* keys, int count, Key* sorted) {
+    if (TEAM > 32 && count <= TEAM / 8) order_by<TEAM, 8>(keys, count, sorted);
+    else if (TEAM > 32 && count <= TEAM / 4) order_by<TEAM, 4>(keys, count, sorted);
+    else order_by<TEAM, TEAM == 32 ? 1 : 2>(keys, count, sorted);
+}
+
+template <int WR>
+struct alignas(16) Picking {
+    // of 64 groups the 32nd largest leaves 64 log 2 = 44 entries above it, of 32 the last one about 32 (1 + 1/2 + ... + 1/32) = 130
+    static constexpr int GROUPS = WR == 1 ? 32 : 64, MEMBERS = 32 * WR / GROUPS, POOL = WR == 1 ? 256 : 128;
+    Key groups[GROUPS], sorted[32], pool[POOL + 2];
+    int in_pool;
+};
+
+// The `top` largest entries of the team's packets [begin, end) (and, in the first CTA, of the row's edges) as a descending list in
+// lists[0], zeros behind them if there are fewer.  seen: the thread's largest entry among its packets; best_batch: the batch of its
+// packets that holds it, -1 if there is nothing but -infinity and NaN.
+template <typename T, int WR>
+__device__ __forceinline__ void top_of_slice(const RowSplit<T>& row, int begin, int end, bool edges, int top, float seen, int best_batch,
+                                             Key (*lists)[32], Picking<WR>& pick, Key* pending) {
+    constexpr int N = Packet<T>::N, TEAM = 32 * WR, MEMBERS = Picking<WR>::MEMBERS;
+    const int t = threadIdx.x % TEAM, lane = t & 31, warp = t >> 5;
     const int n_edges = edges ? row.head + row.tail : 0;
-    // the thread's largest key: its place is looked up in the batch that holds it
-    Key mine = 0;
-    {
-        const int from = best_batch >= 0 ? best_batch : begin + tid;
-        const int until = best_batch >= 0 ? min(end, best_batch + kBatch * kThreads) : end;
-        for (int p = from; p < until; p += kThreads) {
-            const uint4 q = row.packet(p);
-#pragma unroll
-            for (int e = 0; e < N; ++e) mine = max(mine, key_of(entry<T>(q, e), row.first_of(p) + e));
+    const bool has_edge = t < n_edges;
+    const float edge = has_edge ? widen(row.z[row.edge(t)]) : 0.0f;
+    auto packet_at = [&](int p) { return p < end ? row.packet(p) : packet_of_minus_infinity<T>(); };
+    auto entry_key = [&](uint4 q, int p, int e) { return key_of(entry<T>(q, e), row.first_of(p) + e); };
+    enum { BY_VALUE, BY_PLACE, SORTED };
+#pragma unroll 1
+    for (int attempt = BY_VALUE;; ++attempt) {
+        // the thread's largest key (BY_VALUE: told apart by thread, and below any real key of its value)
+        Key mine = 0;
+        if (attempt == BY_VALUE) {
+            if (begin + t < end) mine = (Key)ordered(seen) << 32;
+            if (has_edge) mine = max(mine, (Key)ordered(edge) << 32);
+            if (mine) mine |= (uint32_t)(kThreads - t);
+        } else {
+            const int from = best_batch >= 0 ? best_batch : begin + t, until = best_batch >= 0 ? min(end, best_batch + kBatch * TEAM) : end;
+#pragma unroll 1
+            for (int p = from; p < until; p += TEAM) {
+                const uint4 q = row.packet(p);
+#pragma unroll 1
+                for (int e = 0; e < N; ++e) mine = max(mine, entry_key(q, p, e));
+            }
+            if (has_edge) mine = max(mine, key_of(edge, row.edge(t)));
         }
-        if (tid < n_edges) mine = max(mine, key_of(widen(row.z[row.edge(tid)]), row.edge(tid)));
-    }
-    lists[warp][lane] = sort_down(mine, lane);
-    join_lists(lists, kWarps);
-    const Key tau = max(lists[0][top - 1], (Key)1);
-    const Key chosen = lane < top ? lists[0][lane] : 0;
-    __syncthreads();
-    // a warp reads every kWarps-th of the chosen groups
-    Key best = 0;
-    int waiting = 0;
-    auto offer = [&](Key k) {
-        const bool take = k >= tau;
-        const uint32_t who = __ballot_sync(0xffffffffu, take);
-        if (who == 0) return;
-        if (take) pending[warp][waiting + __popc(who & ((1u << lane) - 1))] = k;
-        waiting += __popc(who);
-        __syncwarp();
-        if (waiting >= 32) {
-            const Key k32 = sort_down(pending[warp][lane], lane);
-            const Key rest = pending[warp][32 + lane];
-            __syncwarp();
-            pending[warp][lane] = rest;
-            const Key other = __shfl_sync(0xffffffffu, k32, 31 - lane);
+        Key group = mine;
+#pragma unroll
+        for (int m = 1; m < MEMBERS; m <<= 1) group = max(group, exchange(group, m));
+        if (t % MEMBERS == 0) pick.groups[t / MEMBERS] = group;
+        if (t < 32) {
+            pick.sorted[t] = 0;
+            lists[0][t] = 0;
+        }
+        if (t == 0) pick.in_pool = 0;
+        team_barrier<WR>();
+        order<TEAM>(pick.groups, Picking<WR>::GROUPS, pick.sorted);
+        team_barrier<WR>();
+        Key tau = pick.sorted[top - 1];
+        if (attempt == BY_VALUE) tau = tau >> 32 << 32;
+        tau = max(tau, (Key)1);
+        // (where tau is a NaN's or nobody's, every entry needs a closer look than its value)
+        const bool all_pass = (tau >> 32) == 0;
+        const uint32_t tau_bits = (uint32_t)(tau >> 32);
+        const float tau_value = __uint_as_float(tau_bits & 0x80000000u ? tau_bits & 0x7fffffffu : ~tau_bits);
+
+        Key best = 0;          // SORTED: the warp's list
+        int waiting = 0;
+        auto flush = [&](Key k) {
+            const Key k32 = sort_down(k, lane), other = __shfl_sync(0xffffffffu, k32, 31 - lane);
             best = merge_down(best > other ? best : other, lane);
-            waiting -= 32;
+        };
+        // one key a lane (0: none): those >= tau to the pool, or to the warp's list
+        auto offer = [&](Key k) {
+            const bool passes = k >= tau;
+            const uint32_t who = __ballot_sync(0xffffffffu, passes);
+            if (who == 0) return;
+            const int before = __popc(who & ((1u << lane) - 1));
+            if (attempt != SORTED) {
+                int at = 0;
+                if (lane == 0) at = atomicAdd(&pick.in_pool, __popc(who));
+                at = __shfl_sync(0xffffffffu, at, 0) + before;
+                if (passes && at < Picking<WR>::POOL) pick.pool[at] = k;
+                return;
+            }
+            if (passes) pending[waiting + before] = k;
+            waiting += __popc(who);
             __syncwarp();
-        }
-    };
-    for (int g = warp; g < top; g += kWarps) {
-        const Key k = __shfl_sync(0xffffffffu, chosen, g);
-        if (k == 0) break;
-        const int index = index_of(k);
-        const bool at_edge = index < row.head || index >= row.head + row.packets * N;
-        const int who = at_edge ? (index < row.head ? index : index - row.packets * N) : ((index - row.head) / N - begin) % kThreads;
-        for (int p0 = begin + who; p0 < end; p0 += 32 * kThreads) {
-            const int p = p0 + lane * kThreads;
-            const bool there = p < end;
-            uint4 q = packet_of_minus_infinity<T>();
-            if (there) q = row.packet(p);
+            if (waiting >= 32) {
+                const Key first = pending[lane], rest = pending[32 + lane];
+                __syncwarp();
+                pending[lane] = rest;
+                flush(first);
+                waiting -= 32;
+                __syncwarp();
+            }
+        };
+        // each lane its own packets, or all lanes one holder's after the other's, kBatch of them under way at a time
+        const uint32_t holders = __ballot_sync(0xffffffffu, mine >= tau);
+        const int per = (end - begin + TEAM - 1) / TEAM;          // packets of a thread
+        const bool own = per <= __popc(holders) * ((per + 31) / 32);
+        const int stride = own ? TEAM : 32 * TEAM;
+        uint32_t left = own ? (per > 0 ? 1u : 0u) : holders;      // what is still to be read: threads (own: all at once)
+        int first = own ? begin + warp * 32 : begin + warp * 32 + __ffs(left) - 1;          // lane 0's packet
+        if (first >= end) left = 0;
+#pragma unroll 1
+        while (left) {
+            uint4 q[kBatch];
+            int at[kBatch];
+            uint32_t bits = 0;
 #pragma unroll
-            for (int e = 0; e < N; ++e) offer(there ? key_of(entry<T>(q, e), row.first_of(p) + e) : 0);
+            for (int i = 0; i < kBatch; ++i) {
+                at[i] = left ? first + (own ? lane : lane * TEAM) : end;
+                q[i] = packet_at(at[i]);
+                first += stride;
+                if (left && first >= end) {
+                    left &= left - 1;
+                    first = begin + warp * 32 + __ffs(left) - 1;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i)
+                if (at[i] < end) bits |= (all_pass ? (1u << N) - 1 : reaching<T>(q[i], tau_value)) << N * i;
+#pragma unroll 1
+            while (__any_sync(0xffffffffu, bits)) {
+                const int bit = __ffs(bits) - 1, i = bit / N, e = bit % N;
+                const uint4 w = i & 2 ? (i & 1 ? q[3] : q[2]) : (i & 1 ? q[1] : q[0]);
+                const int p = i & 2 ? (i & 1 ? at[3] : at[2]) : (i & 1 ? at[1] : at[0]);
+                offer(bits ? entry_key(w, p, e) : 0);
+                bits &= bits - 1;
+            }
         }
-        if (who < n_edges) offer(lane == 0 ? key_of(widen(row.z[row.edge(who)]), row.edge(who)) : 0);
+        if (n_edges > 0 && warp == 0) offer(has_edge ? key_of(edge, row.edge(t)) : 0);
+        if (attempt == SORTED) {
+            flush(lane < waiting ? pending[lane] : 0);
+            lists[warp][lane] = best;
+            join_lists<WR>(lists, WR);
+            return;
+        }
+        team_barrier<WR>();
+        const int count = pick.in_pool;
+        if (count <= Picking<WR>::POOL && (count >= top || attempt == BY_PLACE)) {
+            if (t == 0 && (count & 1)) pick.pool[count] = 0;
+            team_barrier<WR>();
+            order<TEAM>(pick.pool, count, lists[0]);
+            team_barrier<WR>();
+            return;
+        }
+        team_barrier<WR>();          // everybody has read in_pool
     }
-    {
-        const Key k32 = sort_down(lane < waiting ? pending[warp][lane] : 0, lane);
-        const Key other = __shfl_sync(0xffffffffu, k32, 31 - lane);
-        best = merge_down(best > other ? best : other, lane);
-    }
-    lists[warp][lane] = best;
-    join_lists(lists, kWarps);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads) logprobs_kernel(const T* __restrict__ logits, long long ld, long long rows, int vocab,
+template <typename T, int WR, bool TOP>
+__global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const T* __restrict__ logits, long long ld, long long rows, int vocab,
                                                             const int* __restrict__ tokens, float* __restrict__ logprob,
-                                                            float* __restrict__ entropy, float* __restrict__ lse_out, int top,
+                                                            float* __restrict__ entropy, float* __restrict__ lse_out, int top_asked,
                                                             float* __restrict__ top_logprobs, int* __restrict__ top_tokens, int cluster) {
-    constexpr int N = Packet<T>::N;
+    const int top = TOP ? top_asked : 0;
+    constexpr int N = Packet<T>::N, TEAM = 32 * WR, TEAMS = kThreads / TEAM;
     __shared__ Running2 sm[kWarps];
-    __shared__ Running2 from_cta[kMaxCluster];
-    __shared__ Key lists[kMaxCluster][32];
-    __shared__ Key pending[kWarps][64];
-    __shared__ Key from_cta_keys[kMaxCluster][32];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    __shared__ Running2 from_cta[WR == 1 ? 1 : kMaxCluster];
+    __shared__ Key all_lists[WR == 1 ? kWarps : kMaxCluster][32];
+    __shared__ Key pending[TOP ? kWarps : 1][64];
+    __shared__ Key from_cta_keys[WR == 1 ? 1 : kMaxCluster][32];
+    __shared__ Picking<WR> picking[TOP ? TEAMS : 1];
+    const int team = threadIdx.x / TEAM, t = threadIdx.x % TEAM, lane = t & 31, warp = t >> 5;
+    Key(*lists)[32] = all_lists + team * WR;
     const int rank = cluster > 1 ? (int)cluster_rank() : 0;
     if (cluster > 1) cluster_arrive();          // every CTA of the cluster runs before its shared memory is written from another
     dependent_prologue();
     bool started = cluster == 1;
-    for (long long r = blockIdx.x / cluster; r < rows; r += gridDim.x / cluster) {
+    const long long step = (long long)(gridDim.x / cluster) * TEAMS;
+    for (long long r = (long long)(blockIdx.x / cluster) * TEAMS + team; r < rows; r += step) {
         const RowSplit<T> row(logits + r * ld, vocab);
         const int share = (row.packets + cluster - 1) / cluster;
         const int begin = min(row.packets, rank * share), end = min(row.packets, begin + share);
@@ -420,26 +557,30 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const T* __restrict_
         {
             Two s2 = two(0, 0), u2 = two(0, 0);
             auto raise = [&](float to) {
-                float a, b, c, d;
-                parts(s2, a, b);
-                parts(u2, c, d);
-                me.s = a + b;
-                me.u = c + d;
+                me.s = total(s2);
+                me.u = total(u2);
                 me.raise(to);
                 s2 = two(me.s, 0);
                 u2 = two(me.u, 0);
             };
-            for (int b = begin + tid; b < end; b += kBatch * kThreads) {
+            uint4 ahead[kBatch];          // the next batch is on its way while one is worked on
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) ahead[i] = begin + t + i * TEAM < end ? row.packet(begin + t + i * TEAM) : packet_of_minus_infinity<T>();
+            for (int b = begin + t; b < end; b += kBatch * TEAM) {
                 uint4 q[kBatch];
 #pragma unroll
-                for (int i = 0; i < kBatch; ++i) q[i] = b + i * kThreads < end ? row.packet(b + i * kThreads) : packet_of_minus_infinity<T>();
+                for (int i = 0; i < kBatch; ++i) {
+                    q[i] = ahead[i];
+                    const int p = b + (kBatch + i) * TEAM;
+                    ahead[i] = p < end ? row.packet(p) : packet_of_minus_infinity<T>();
+                }
                 const float high = largest(q, (T*)nullptr);
                 if (high > seen) {
                     seen = high;
                     best_batch = b;
                     if (high > me.m) raise(high);
                 }
-                const Two minus = two(-me.m, -me.m), scale = two(kLog2e, kLog2e);
+                const Two minus = both(-me.m), scale = both(kLog2e);
 #pragma unroll
                 for (int i = 0; i < kBatch; ++i) {
                     Two z[N / 2];
@@ -456,37 +597,32 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const T* __restrict_
                     }
                 }
             }
-            if (rank == 0 && tid < row.head + row.tail) {
-                const float z = widen(row.z[row.edge(tid)]);
+            if (rank == 0 && t < row.head + row.tail) {
+                const float z = widen(row.z[row.edge(t)]);
                 if (z > me.m) raise(z);
-                const float t = max_nan((z - me.m) * kLog2e, kFloor), p = exp2_of(t);
+                const float d = max_nan((z - me.m) * kLog2e, kFloor), p = exp2_of(d);
                 s2 = s2 + two(p, 0);
-                u2 = u2 + two(t * p, 0);
+                u2 = u2 + two(d * p, 0);
             }
-            raise(me.m);
+            me.s = total(s2);
+            me.u = total(u2);
         }
-#pragma unroll
-        for (int m = 16; m > 0; m >>= 1) {
-            Running2 o;
-            o.m = __shfl_xor_sync(0xffffffffu, me.m, m);
-            o.s = __shfl_xor_sync(0xffffffffu, me.s, m);
-            o.u = __shfl_xor_sync(0xffffffffu, me.u, m);
-            me.merge(o);
+        me.over_lanes<32>();
+        if (WR > 1) {
+            __syncthreads();          // the row before has been written
+            if (lane == 0) sm[warp] = me;
         }
-        __syncthreads();          // the row before has been written
-        if (lane == 0) sm[warp] = me;
-        if (top > 0) top_of_slice(row, begin, end, rank == 0, top, best_batch, lists, pending);
-        else __syncthreads();
-        if (cluster > 1) {
+        if constexpr (TOP) top_of_slice<T, WR>(row, begin, end, rank == 0, top, seen, best_batch, lists, picking[team], pending[threadIdx.x >> 5]);
+        else if (WR > 1) __syncthreads();
+        if (WR > 1 && cluster > 1) {
             if (!started) { cluster_wait(); started = true; }
             if (warp == 0) {
+                me = sm[lane % kWarps];
+                me.over_lanes<kWarps>();
                 if (lane == 0) {
-                    Running2 all = sm[0];
-#pragma unroll
-                    for (int w = 1; w < kWarps; ++w) all.merge(sm[w]);
-                    store_remote(in_first_cta(&from_cta[rank].m), all.m);
-                    store_remote(in_first_cta(&from_cta[rank].s), all.s);
-                    store_remote(in_first_cta(&from_cta[rank].u), all.u);
+                    store_remote(in_first_cta(&from_cta[rank].m), me.m);
+                    store_remote(in_first_cta(&from_cta[rank].s), me.s);
+                    store_remote(in_first_cta(&from_cta[rank].u), me.u);
                 }
                 if (top > 0) store_remote(in_first_cta(&from_cta_keys[rank][lane]), lists[0][lane]);
             }
@@ -494,27 +630,34 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const T* __restrict_
             cluster_wait();
             if (rank == 0 && top > 0) {
                 for (int w = warp; w < cluster; w += kWarps) lists[w][lane] = from_cta_keys[w][lane];
-                join_lists(lists, cluster);
+                join_lists<WR>(lists, cluster);
             }
         }
         if (rank == 0 && warp == 0) {
-            Running2 all = cluster > 1 ? from_cta[0] : sm[0];
-            for (int w = 1; w < (cluster > 1 ? cluster : kWarps); ++w) all.merge(cluster > 1 ? from_cta[w] : sm[w]);
+            if (WR > 1 && cluster > 1) {
+                me = from_cta[lane % cluster];          // (every CTA's sums 32 / cluster times)
+                me.over_lanes<32>();
+                me.s *= cluster * (1.0f / 32);
+                me.u *= cluster * (1.0f / 32);
+            } else if (WR > 1) {
+                me = sm[lane % kWarps];
+                me.over_lanes<kWarps>();
+            }
             float l, h;
-            if (all.s == 0) {          // nothing but -infinity
+            if (me.s == 0) {          // nothing but -infinity
                 l = -infinity_of(0.0f);
                 h = 0;
             } else {
-                const float ls = logf(all.s);
-                l = all.m + ls;
-                h = ls - kLn2 * (all.u / all.s);
+                const float ls = logf(me.s);
+                l = me.m + ls;
+                h = ls - kLn2 * (me.u / me.s);
             }
             if (lane == 0) {
                 if (entropy) entropy[r] = h;
                 if (lse_out) lse_out[r] = l;
                 if (logprob) {
-                    const int t = tokens[r];
-                    logprob[r] = t < 0 ? 0.0f : t >= vocab ? nan_of(0.0f) : log_p(widen(row.z[t]), l);
+                    const int given = tokens[r];
+                    logprob[r] = given < 0 ? 0.0f : given >= vocab ? nan_of(0.0f) : log_p(widen(row.z[given]), l);
                 }
             }
             if (lane < top) {
@@ -523,7 +666,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_kernel(const T* __restrict_
                 top_logprobs[r * top + lane] = log_p(widen(row.z[index]), l);
             }
         }
-        if (cluster > 1) {           // the first CTA has read what the others sent for this row
+        if (WR > 1 && cluster > 1) {           // the first CTA has read what the others sent for this row
             cluster_arrive();
             cluster_wait();
         }
@@ -632,22 +775,29 @@ long long capped(long long want, long long most) { return std::max<long long>(1,
 template <typename T>
 cudaError_t forward(cudaStream_t s, const Rows& z, const int* tokens, void* logprob, void* entropy, void* lse, int top, void* top_logprobs,
                     int* top_tokens) {
-    // as many CTAs a row as fill the machine, none with less than one batch of packets for its threads
+    // A warp per row where that is a few batches for it, or where there are rows for every warp of the machine (16384 x 8192 bf16: 49 us, a
+    // CTA per row 89); else a CTA per row, and several for so few rows that two CTAs a SM are not reached with one (64 x 131072 bf16:
+    // 9 us with eight, 20 with one; 1000 x 50001 f32: 35 us with one, 48 with two), none with less than one batch for its
+    // threads.
     const long long packets = z.cols / Packet<T>::N;
+    const bool warp_each = packets <= 32 * kBatch * 2 || (packets <= 32 * kBatch * 8 && z.rows >= kSms * 8);
     int cluster = 1;
-    while (cluster < kMaxCluster && z.rows * cluster < kSms * 8 && packets >= 2ll * cluster * kBatch * kThreads) cluster *= 2;
+    while (!warp_each && cluster < kMaxCluster && z.rows * cluster <= kSms * 2 && packets >= 2ll * cluster * kBatch * kThreads) cluster *= 2;
+    auto kernel = warp_each ? (top ? logprobs_kernel<T, 1, true> : logprobs_kernel<T, 1, false>)
+                            : (top ? logprobs_kernel<T, kWarps, true> : logprobs_kernel<T, kWarps, false>);
     if (cluster > 8) {
-        static std::atomic<unsigned long long> allowed(0);      // by device
+        static std::atomic<unsigned long long> allowed[2];      // by device
         int device = 0;
         cudaError_t e = cudaGetDevice(&device);
-        if (e == cudaSuccess && !(allowed.load() >> (device & 63) & 1)) {
-            e = cudaFuncSetAttribute(logprobs_kernel<T>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-            if (e == cudaSuccess) allowed.fetch_or(1ull << (device & 63));
+        if (e == cudaSuccess && !(allowed[top > 0].load() >> (device & 63) & 1)) {
+            e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+            if (e == cudaSuccess) allowed[top > 0].fetch_or(1ull << (device & 63));
         }
         if (e != cudaSuccess) return e;
     }
-    const long long clusters = std::min<long long>(z.rows, (1ll << 30) / cluster);
-    return launch(logprobs_kernel<T>, dim3((unsigned)(clusters * cluster)), kThreads, 0, s, cluster, (const T*)z.data, (long long)z.stride,
+    const int teams = warp_each ? kWarps : 1;
+    const long long clusters = std::min<long long>((z.rows + teams - 1) / teams, (1ll << 30) / cluster);
+    return launch(kernel, dim3((unsigned)(clusters * cluster)), kThreads, 0, s, cluster, (const T*)z.data, (long long)z.stride,
                   (long long)z.rows, (int)z.cols, tokens, (float*)logprob, (float*)entropy, (float*)lse, top, (float*)top_logprobs, top_tokens,
                   cluster);
 }
