@@ -21,7 +21,7 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kList = 96;                    // tensors a launch takes (a list of 96 stays within 4 KB of kernel parameters)
-constexpr int kChunk = 16384;                // elements
+constexpr int kMinChunk = 2048, kMaxChunk = 65536;      // elements
 constexpr int kMaxCtas = kSms * 8;
 
 struct List {
@@ -30,7 +30,7 @@ struct List {
     long long numel[kList];
     long long first[kList + 1];              // chunk
     unsigned char dtype[kList];
-    int n;
+    int n, chunk;
 };
 
 // the tensor that holds a chunk
@@ -49,39 +49,59 @@ constexpr int kBatch = 4;                    // packets a thread has under way
 __device__ __forceinline__ double square(double s, float v) { const double d = (double)v; return fma(d, d, s); }
 __device__ __forceinline__ double square(double s, double v) { return fma(v, v, s); }
 
+// a thread's packets of a piece of memory: `head` elements up to the 16-byte grid, whole packets, the rest
+template <typename T>
+struct Piece {
+    static constexpr int N = Packet<T>::N;
+    const T* body;
+    int head, packets, edges;
+    __device__ __forceinline__ Piece(const T* x, int n) {
+        head = min(n, (int)((16 - (uintptr_t)x % 16) % 16 / sizeof(T)));
+        packets = (n - head) / N;
+        edges = n - packets * N;
+        body = x + head;
+    }
+    // place of the thread's edge element in the piece (threadIdx.x < edges)
+    __device__ __forceinline__ int edge() const { return (int)threadIdx.x < head ? threadIdx.x : threadIdx.x + packets * N; }
+    __device__ __forceinline__ Packet<T> packet(int p) const {
+        Packet<T> q = {};
+        if (p < packets) q = load_packet(body + p * N);
+        return q;
+    }
+};
+
 template <typename T>
 __device__ __forceinline__ double sum_chunk(const T* x, int n) {
     constexpr int N = Packet<T>::N;
-    const int head = min(n, (int)((16 - (uintptr_t)x % 16) % 16 / sizeof(T))), packets = (n - head) / N, edges = n - packets * N;
-    const T* body = x + head;
+    const Piece<T> piece(x, n);
     double s = 0, s2 = 0;
-    if ((int)threadIdx.x < edges) s = square(s, widen(x[(int)threadIdx.x < head ? threadIdx.x : threadIdx.x + packets * N]));
-    for (int p = threadIdx.x; p < packets; p += kBatch * kThreads) {
-        Packet<T> q[kBatch];
+    if ((int)threadIdx.x < piece.edges) s = square(s, widen(x[piece.edge()]));
+    Packet<T> ahead[kBatch];          // the next packets are on their way while some are worked on (absent ones are zeros)
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i)
-            if (p + i * kThreads < packets) q[i] = load_packet(body + (p + i * kThreads) * N);
+    for (int i = 0; i < kBatch; ++i) ahead[i] = piece.packet(threadIdx.x + i * kThreads);
+    for (int p = threadIdx.x; p < piece.packets; p += kBatch * kThreads) {
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i)
-            if (p + i * kThreads < packets) {
+        for (int i = 0; i < kBatch; ++i) {
+            const Packet<T> q = ahead[i];
+            ahead[i] = piece.packet(p + (kBatch + i) * kThreads);
 #pragma unroll
-                for (int e = 0; e < N; e += 2) {
-                    s = square(s, widen(q[i].v[e]));
-                    s2 = square(s2, widen(q[i].v[e + 1]));
-                }
+            for (int e = 0; e < N; e += 2) {
+                s = square(s, widen(q.v[e]));
+                s2 = square(s2, widen(q.v[e + 1]));
             }
+        }
     }
     return s + s2;
 }
 
-__global__ void __launch_bounds__(kThreads) squares_kernel(const __grid_constant__ List l, double* __restrict__ partial) {
+__global__ void __launch_bounds__(kThreads, 4) squares_kernel(const __grid_constant__ List l, double* __restrict__ partial) {
     __shared__ double sm[kThreads / 32];
     dependent_prologue();
     double s = 0;
     for (long long c = blockIdx.x; c < l.first[l.n]; c += gridDim.x) {
         const int t = tensor_of(l, c);
-        const long long at = (c - l.first[t]) * kChunk;
-        const int n = (int)min((long long)kChunk, l.numel[t] - at);
+        const long long at = (c - l.first[t]) * l.chunk;
+        const int n = (int)min((long long)l.chunk, l.numel[t] - at);
         if (l.dtype[t] == DALIB200_F32) s += sum_chunk((const float*)l.in[t] + at, n);
         else if (l.dtype[t] == DALIB200_BF16) s += sum_chunk((const bf16_s*)l.in[t] + at, n);
         else s += sum_chunk((const double*)l.in[t] + at, n);
@@ -119,27 +139,24 @@ __device__ __forceinline__ void scale_chunk(const T* x, T* y, int n, F f) {
         for (int i = threadIdx.x; i < n; i += kThreads) y[i] = Narrow<T>::of(widen(x[i]) * f);
         return;
     }
-    const int head = min(n, (int)((16 - (uintptr_t)x % 16) % 16 / sizeof(T))), packets = (n - head) / N, edges = n - packets * N;
-    if ((int)threadIdx.x < edges) {
-        const int i = (int)threadIdx.x < head ? threadIdx.x : threadIdx.x + packets * N;
-        y[i] = Narrow<T>::of(widen(x[i]) * f);
-    }
-    for (int p = threadIdx.x; p < packets; p += kBatch * kThreads) {
+    const Piece<T> piece(x, n);
+    if ((int)threadIdx.x < piece.edges) y[piece.edge()] = Narrow<T>::of(widen(x[piece.edge()]) * f);
+    for (int p = threadIdx.x; p < piece.packets; p += kBatch * kThreads) {
         Packet<T> q[kBatch];
 #pragma unroll
-        for (int i = 0; i < kBatch; ++i)
-            if (p + i * kThreads < packets) q[i] = load_packet(x + head + (p + i * kThreads) * N);
+        for (int i = 0; i < kBatch; ++i) q[i] = piece.packet(p + i * kThreads);
 #pragma unroll
         for (int i = 0; i < kBatch; ++i)
-            if (p + i * kThreads < packets) {
+            if (p + i * kThreads < piece.packets) {
 #pragma unroll
                 for (int e = 0; e < N; ++e) q[i].v[e] = Narrow<T>::of(widen(q[i].v[e]) * f);
-                store_packet(y + head + (p + i * kThreads) * N, q[i]);
+                // (streaming: what is written is not read here again, what is still in L2 of the first pass is)
+                __stcs(reinterpret_cast<uint4*>(y + piece.head + (p + i * kThreads) * N), *reinterpret_cast<const uint4*>(&q[i]));
             }
     }
 }
 
-__global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__ List l, const double* __restrict__ partial, int n_partial,
+__global__ void __launch_bounds__(kThreads, 4) scale_kernel(const __grid_constant__ List l, const double* __restrict__ partial, int n_partial,
                                                          double max_norm, void* norm, int norm_f64) {
     __shared__ double sm[kThreads / 32];
     dependent_prologue();
@@ -152,8 +169,8 @@ __global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__
     for (long long c = l.first[l.n] - 1 - blockIdx.x; c >= 0; c -= gridDim.x) {
         const int t = tensor_of(l, c);
         if (!down && l.in[t] == l.out[t]) continue;
-        const long long at = (c - l.first[t]) * kChunk;
-        const int m = (int)min((long long)kChunk, l.numel[t] - at);
+        const long long at = (c - l.first[t]) * l.chunk;
+        const int m = (int)min((long long)l.chunk, l.numel[t] - at);
         if (l.dtype[t] == DALIB200_F32) scale_chunk((const float*)l.in[t] + at, (float*)l.out[t] + at, m, (float)f);
         else if (l.dtype[t] == DALIB200_BF16) scale_chunk((const bf16_s*)l.in[t] + at, (bf16_s*)l.out[t] + at, m, (float)f);
         else scale_chunk((const double*)l.in[t] + at, (double*)l.out[t] + at, m, f);
@@ -181,6 +198,11 @@ std::string gather_list(int n, const int* dtypes, const int64_t* numel, const vo
     if (n > 0 && (!dtypes || !numel || !in)) return "the list's dtypes, numel or pointers are null";
     std::vector<Range> ranges;
     List* l = nullptr;
+    // chunks of a size that gives every CTA several, and of one packet a thread at least
+    int64_t all = 0;
+    for (int i = 0; i < n; ++i) all += numel[i] > 0 ? std::min<int64_t>(numel[i], int64_t(1) << 40) : 0;
+    int chunk = kMinChunk;
+    while (chunk < kMaxChunk && (int64_t)chunk * kMaxCtas * 4 < all) chunk *= 2;
     for (int i = 0; i < n; ++i) {
         const std::string who = "tensor " + std::to_string(i);
         if (!floating(dtypes[i])) return who + ": dtype must be f32, f64 or bf16";
@@ -198,6 +220,7 @@ std::string gather_list(int n, const int* dtypes, const int64_t* numel, const vo
             t->lists.emplace_back();
             l = &t->lists.back();
             l->n = 0;
+            l->chunk = chunk;
             l->first[0] = 0;
         }
         const int k = l->n++;
@@ -205,7 +228,7 @@ std::string gather_list(int n, const int* dtypes, const int64_t* numel, const vo
         l->out[k] = out ? out[i] : nullptr;
         l->numel[k] = numel[i];
         l->dtype[k] = (unsigned char)dtypes[i];
-        l->first[k + 1] = l->first[k] + (numel[i] + kChunk - 1) / kChunk;
+        l->first[k + 1] = l->first[k] + (numel[i] + chunk - 1) / chunk;
     }
     // what is written is read or written nowhere else in the list
     std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.lo < b.lo; });
