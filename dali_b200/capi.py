@@ -280,7 +280,7 @@ class Library:
     # -- operators of a token model (arguments that are None are left out, workspace: a CUDA tensor or None) ----------
     @staticmethod
     def _address(x):
-        return None if x is None else x.data_ptr() if hasattr(x, "data_ptr") else int(x)
+        return x if x is None or type(x) is int else x.data_ptr()
 
     @staticmethod
     def _workspace(w):
@@ -321,12 +321,15 @@ class Library:
             device, stream, dtype, rows, vocab, a(logits), vocab if row_stride is None else row_stride, a(tokens), a(lse), a(entropy),
             a(dlogprob), a(dentropy), a(dlogits), vocab if dlogits_row_stride is None else dlogits_row_stride))
 
+    @staticmethod
+    def _addresses(tensors):
+        return (_P * len(tensors))(*[x if x is None or type(x) is int else x.data_ptr() for x in tensors])
+
     def _tensor_list(self, dtypes, numel, tensors):
         n = len(tensors)
         if len(dtypes) != n or len(numel) != n:
             raise ValueError("dtypes, numel and tensors must have one entry per tensor")
-        a = self._address
-        return n, (_I * n)(*dtypes), (_L * n)(*numel), (_P * n)(*[a(x) for x in tensors])
+        return n, (_I * n)(*dtypes), (_L * n)(*numel), self._addresses(tensors)
 
     def sum_squares(self, dtypes, numel, tensors, out, workspace=None, device=0, stream=None):
         """*out (fp64) = sum of the squares of all elements of a list of contiguous tensors."""
@@ -341,7 +344,7 @@ class Library:
     def _outs(self, n, outs):
         if len(outs) != n:
             raise ValueError("outs must have one entry per tensor")
-        return (_P * n)(*[self._address(x) for x in outs])
+        return self._addresses(outs)
 
     def scale_to_norm(self, dtypes, numel, tensors, outs, sum_squares, max_norm, device=0, stream=None):
         """outs[i] = tensors[i] * min(1, max_norm / sqrt(*sum_squares))."""

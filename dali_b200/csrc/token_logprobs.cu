@@ -385,7 +385,7 @@ template <int WR>
 struct alignas(16) Picking {
     // of 64 groups the 32nd largest leaves 64 log 2 = 44 entries above it, of 32 the last one about 32 (1 + 1/2 + ... + 1/32) = 130
     static constexpr int GROUPS = WR == 1 ? 32 : 64, MEMBERS = 32 * WR / GROUPS, POOL = WR == 1 ? 256 : 128;
-    Key groups[GROUPS], sorted[32], pool[POOL + 2];
+    Key groups[WR == 1 ? 2 : GROUPS], sorted[WR == 1 ? 2 : 32], pool[POOL + 2];
     int in_pool;
 };
 
@@ -424,16 +424,22 @@ __device__ __forceinline__ void top_of_slice(const RowSplit<T>& row, int begin, 
         Key group = mine;
 #pragma unroll
         for (int m = 1; m < MEMBERS; m <<= 1) group = max(group, exchange(group, m));
-        if (t % MEMBERS == 0) pick.groups[t / MEMBERS] = group;
-        if (t < 32) {
-            pick.sorted[t] = 0;
-            lists[0][t] = 0;
-        }
         if (t == 0) pick.in_pool = 0;
-        team_barrier<WR>();
-        order<TEAM>(pick.groups, Picking<WR>::GROUPS, pick.sorted);
-        team_barrier<WR>();
-        Key tau = pick.sorted[top - 1];
+        Key tau;
+        if constexpr (WR == 1) {
+            tau = __shfl_sync(0xffffffffu, sort_down(group, lane), top - 1);
+            __syncwarp();
+        } else {
+            if (t % MEMBERS == 0) pick.groups[t / MEMBERS] = group;
+            if (t < 32) {
+                pick.sorted[t] = 0;
+                lists[0][t] = 0;
+            }
+            team_barrier<WR>();
+            order<TEAM>(pick.groups, Picking<WR>::GROUPS, pick.sorted);
+            team_barrier<WR>();
+            tau = pick.sorted[top - 1];
+        }
         if (attempt == BY_VALUE) tau = tau >> 32 << 32;
         tau = max(tau, (Key)1);
         // (where tau is a NaN's or nobody's, every entry needs a closer look than its value)
@@ -517,6 +523,12 @@ __device__ __forceinline__ void top_of_slice(const RowSplit<T>& row, int begin, 
         team_barrier<WR>();
         const int count = pick.in_pool;
         if (count <= Picking<WR>::POOL && (count >= top || attempt == BY_PLACE)) {
+            if constexpr (WR == 1) {          // (a warp sorts and merges faster than it counts)
+                for (int i = 0; i < count; i += 32) flush(i + lane < count ? pick.pool[i + lane] : 0);
+                lists[0][lane] = best;
+                __syncwarp();
+                return;
+            }
             if (t == 0 && (count & 1)) pick.pool[count] = 0;
             team_barrier<WR>();
             order<TEAM>(pick.pool, count, lists[0]);
