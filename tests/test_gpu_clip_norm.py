@@ -152,6 +152,32 @@ def test_the_same_call_gives_the_same_bits(lib):
         assert all(torch.equal(a, b) for a, b in zip(seen[0], other))
 
 
+def test_threads_that_share_a_stream_and_the_library_space(lib):
+    import threading
+    rng = np.random.default_rng(9)
+    specs = [[(300001, F32), (5, BF16)], [(4000000, BF16)], [(1000 + i, F32) for i in range(150)], [(70, F64)]]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    tensors = [tensors_of(rng, s) for s in specs]
+    want = [norm_of(t) for t in tensors]
+    norms = [torch.zeros((), device="cuda") for _ in specs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def loop(k):
+        d, n = [x for _, x in specs[k]], [x for x, _ in specs[k]]
+        for _ in range(30):
+            lib.global_norm(d, n, tensors[k], norms[k], stream=streams[k // 2].cuda_stream)
+            lib.sync(stream=streams[k // 2].cuda_stream)
+            if abs(norms[k].item() - want[k]) > want[k] * (2.0 ** -24 + 1e-12):
+                wrong.append((k, norms[k].item(), want[k]))
+    threads = [threading.Thread(target=loop, args=(k,)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+
+
 def test_streams_and_graphs(lib):
     rng = np.random.default_rng(4)
     spec = [(100003, F32), (77, BF16)] * 60

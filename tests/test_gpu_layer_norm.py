@@ -115,6 +115,14 @@ def test_backward(lib, shape, types):
 
 
 @pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("shape", [(3, 9001), (2, 12000), (3, 16384), (2, 16383), (1200, 100), (2500, 8), (900, 520), (450, 2047), (301, 4100)])
+def test_long_rows_and_many_rows(lib, shape, types):
+    """Rows that 8 or 16 warps share, and more rows than a grid takes at once, on the 16-byte grid and off it."""
+    test_forward(lib, shape, types)
+    test_backward(lib, shape, types)
+
+
+@pytest.mark.parametrize("types", TYPES)
 @pytest.mark.parametrize("rows,cols", [(6, 1000), (150, 1024), (5, 513), (700, 96), (3, 33000)])
 def test_strides_offsets_and_writing_over_an_input(lib, rows, cols, types):
     dt, wt = types
@@ -301,6 +309,82 @@ def test_streams_and_graphs(lib):
         with pytest.raises(DaliB200Error, match="workspace"):
             both(0, torch.cuda.current_stream().cuda_stream, None)
     del graphs, g
+
+
+def test_matrices_whose_rows_do_not_lie_alike(lib):
+    """x, dy and dx each start elsewhere in a 16-byte packet, and their strides differ by odd numbers."""
+    rng = np.random.default_rng(12)
+    for dt in (F32, BF16, F64):
+        for rows, cols in ((40, 100), (9, 2050), (3, 9000)):
+            _, x = matrix(rng, rows, cols, dt, cols + 1, 1)
+            _, dy = matrix(rng, rows, cols, dt, cols + 4, 2)
+            _, dx = matrix(rng, rows, cols, dt, cols + 7, 3)
+            dg, db = (torch.empty(cols, device="cuda", dtype=TORCH[dt]) for _ in range(2))
+            f = Formula(x, None, None, dt)
+            want = f.grads(dy, rows)
+            lib.layer_norm_backward(dt, dt, rows, cols, dy, x, None, dx, dg, db, eps=EPS, dy_row_stride=cols + 4, x_row_stride=cols + 1,
+                                    dx_row_stride=cols + 7)
+            for got, w in zip((dx, dg, db), want):
+                agree(got, *w, dt)
+            lib.layer_norm(dt, dt, rows, cols, x, None, None, dx, eps=EPS, x_row_stride=cols + 1, out_row_stride=cols + 7)
+            agree(dx, *f.y(), dt)
+
+
+def test_weights_off_the_grid(lib):
+    rng = np.random.default_rng(13)
+    for dt, wt in TYPES:
+        for cols in (256, 1000, 4096, 8192, 20000):
+            _, x = matrix(rng, 5, cols, dt)
+            _, dy = matrix(rng, 5, cols, dt)
+            both = torch.from_numpy(1 + 0.3 * rng.standard_normal(2 * cols + 3)).cuda().to(TORCH[wt])
+            gamma, beta = both[1:1 + cols], both[cols + 3:2 * cols + 3]
+            grads = torch.full((2 * cols + 3,), 7.0, device="cuda", dtype=TORCH[wt])
+            out = torch.empty_like(x)
+            lib.layer_norm(dt, wt, 5, cols, x, gamma, beta, out, eps=EPS)
+            f = Formula(x, gamma, beta, dt)
+            agree(out, *f.y(), dt)
+            lib.layer_norm_backward(dt, wt, 5, cols, dy, x, gamma, out, grads[1:1 + cols], grads[cols + 3:2 * cols + 3], eps=EPS)
+            want = f.grads(dy, 5)
+            for got, w, t in zip((out, grads[1:1 + cols], grads[cols + 3:2 * cols + 3]), want, (dt, wt, wt)):
+                agree(got, *w, t)
+            assert grads[0] == 7 and (grads[1 + cols:cols + 3] == 7).all()
+
+
+def test_threads_that_share_a_stream_and_the_library_space(lib):
+    """Four host threads, two of them on one stream, all of them without a workspace of their own."""
+    import threading
+    rng = np.random.default_rng(14)
+    shapes = [(700, 1024), (60, 4096), (900, 300), (33, 9000)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    work = []
+    for rows, cols in shapes:
+        _, x = matrix(rng, rows, cols, F32)
+        _, dy = matrix(rng, rows, cols, F32)
+        work.append((rows, cols, x, dy, [torch.empty(cols, device="cuda") for _ in range(2)]))
+    torch.cuda.synchronize()
+    wrong = []
+
+    def loop(k):
+        rows, cols, x, dy, (dg, db) = work[k]
+        first = None
+        for _ in range(30):
+            lib.layer_norm_backward(F32, F32, rows, cols, dy, x, None, None, dg, db, stream=streams[k // 2].cuda_stream)
+            lib.sync(stream=streams[k // 2].cuda_stream)
+            now = (dg.cpu(), db.cpu())
+            if first is None:
+                first = now
+            elif not all(torch.equal(a, b) for a, b in zip(first, now)):
+                wrong.append(k)
+    threads = [threading.Thread(target=loop, args=(k,)) for k in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    for rows, cols, x, dy, (dg, db) in work:
+        want = Formula(x, None, None, F32).grads(dy, rows)
+        agree(dg, *want[1], F32)
+        agree(db, *want[2], F32)
 
 
 def test_a_workspace_that_is_too_small_is_refused(lib):

@@ -197,6 +197,46 @@ def test_rows_that_are_not_numbers(lib, vocab, dt):
     assert (tt >= 0).all() and (tt < vocab).all()
 
 
+@pytest.mark.parametrize("dt", [F32, BF16])
+@pytest.mark.parametrize("rows,vocab", [(1, 40000), (400, 40000), (1300, 4096), (3, 1500)])
+@pytest.mark.parametrize("top", [1, 5, 32])
+def test_the_largest_entries_lie_together(lib, rows, vocab, top, dt):
+    """More large entries in the packets of a few threads than any other thread's largest: the alternatives are then sorted, not
+    counted.  Which threads those are depends on the team: every 16th packet of a row is large, the first 40, or the last 40."""
+    rng = np.random.default_rng(vocab + top)
+    _, z = logits_of(rng, rows, vocab, dt)
+    per = 16 // z.element_size()
+    packet = torch.arange(vocab, device="cuda") // per
+    for far in (packet % 256 < 4, packet % 32 == 0, packet < 40, packet >= (vocab - 1) // per - 40):
+        y = torch.where(far, z + 40, z)
+        if rows == 1300:
+            y = y[:1200]
+        tokens = torch.zeros(y.shape[0], dtype=torch.int32, device="cuda")
+        check_forward(lib, dt, y.contiguous(), tokens, top)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16, F64])
+@pytest.mark.parametrize("rows,vocab", [(2, 40), (2, 3000), (400, 3000), (1, 70000), (1500, 2048)])
+def test_fewer_numbers_than_alternatives(lib, rows, vocab, dt):
+    """Rows of NaN with 3 numbers, of -infinity with 3 numbers, of both: numbers first, then -infinity, then NaN, each by index."""
+    rng = np.random.default_rng(vocab)
+    for kind in range(3):
+        z = torch.full((rows, vocab), (float("nan"), -INF, float("nan"))[kind], device="cuda", dtype=TORCH[dt])
+        if kind == 2:
+            z[:, vocab // 2:] = -INF
+        at = torch.from_numpy(np.stack([rng.permutation(vocab)[:3] for _ in range(rows)])).cuda()
+        z.scatter_(1, at, torch.tensor([1.0, 2.0, 2.0], device="cuda", dtype=TORCH[dt]).expand(rows, 3).contiguous())
+        tokens = torch.zeros(rows, dtype=torch.int32, device="cuda")
+        _, _, lse, tl, tt = forward(lib, dt, z, tokens, 10)
+        rank = torch.where(torch.isnan(z), -2.0, torch.where(torch.isinf(z), -1.0, z.double()))
+        want = torch.sort(rank, dim=1, descending=True, stable=True).indices[:, :10]
+        assert torch.equal(tt.long(), want)
+        if kind == 1:
+            check_forward(lib, dt, z, tokens, 10)
+        else:
+            assert torch.isnan(lse).all() and torch.isnan(tl).all()
+
+
 @pytest.mark.parametrize("dt", [F32, BF16, F64])
 @pytest.mark.parametrize("vocab", [64, 777, 20000, 66001])
 def test_strides_and_offsets(lib, vocab, dt):
