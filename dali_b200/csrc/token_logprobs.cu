@@ -728,14 +728,27 @@ __global__ void __launch_bounds__(kThreads) logprobs_backward_kernel(const T* lo
                                                                      const float* __restrict__ dentropy, T* dlogits, long long ldd) {
     constexpr int N = Packet<T>::N;
     dependent_prologue();
+    // what a row's entries need, read a piece ahead: the packets can be asked for at once
+    struct Row { int t; float g, l, w, h; };
+    auto row_of = [&](long long piece) {
+        const long long r = piece / per_row;
+        Row v;
+        v.t = dlogprob ? tokens[r] : -1;
+        v.g = dlogprob ? dlogprob[r] : 0.0f;
+        v.l = lse[r];
+        v.w = ENTROPY ? dentropy[r] : 0.0f;
+        v.h = ENTROPY ? entropy[r] : 0.0f;
+        return v;
+    };
+    Row next = row_of(blockIdx.x);
     for (long long piece = blockIdx.x; piece < pieces; piece += gridDim.x) {
         const long long r = piece / per_row;
         const int part = (int)(piece - r * per_row);
         const RowSplit<T> row(logits + r * ld, vocab);
         T* out = dlogits + r * ldd;
-        const int t = dlogprob ? tokens[r] : -1;
-        const float g = t < 0 ? 0.0f : t >= vocab ? nan_of(0.0f) : dlogprob[r], l = lse[r];
-        const float w = ENTROPY ? dentropy[r] : 0.0f, h = ENTROPY ? entropy[r] : 0.0f;
+        const int t = next.t;
+        const float g = t < 0 ? 0.0f : t >= vocab ? nan_of(0.0f) : next.g, l = next.l, w = next.w, h = next.h;
+        if (piece + gridDim.x < pieces) next = row_of(piece + gridDim.x);
         const bool nothing = (g == 0 && w == 0) || l == -infinity_of(0.0f);
         const float a = -(g + w * h), b = -w * kLn2;
         const int begin = part * kBatch * kThreads + threadIdx.x;
@@ -772,7 +785,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_backward_kernel(const T* lo
 #pragma unroll
                 for (int e = 0; e < N / 2; ++e) z[e] = z[e] + two(j == 2 * e ? g : 0.0f, j == 2 * e + 1 ? g : 0.0f);
             }
-            *reinterpret_cast<uint4*>(out + row.first_of(p)) = packet_of(z, (const T*)nullptr);
+            __stcs(reinterpret_cast<uint4*>(out + row.first_of(p)), packet_of(z, (const T*)nullptr));
         }
         if (part == 0 && (int)threadIdx.x < row.head + row.tail) {
             const int j = row.edge(threadIdx.x);
@@ -831,7 +844,7 @@ cudaError_t backward(cudaStream_t s, const Rows& z, const int* tokens, const voi
         if (alike) {
             const long long packets = z.cols / Packet<T>::N, per_row = std::max<long long>(1, (packets + kBatch * kThreads - 1) / (kBatch * kThreads));
             const long long pieces = z.rows * per_row;
-            return launch(dentropy ? logprobs_backward_kernel<T, true> : logprobs_backward_kernel<T, false>, dim3((unsigned)capped(pieces, 1 << 30)),
+            return launch(dentropy ? logprobs_backward_kernel<T, true> : logprobs_backward_kernel<T, false>, dim3((unsigned)capped(pieces, kSms * 8)),
                           kThreads, 0, s, 1, (const T*)z.data, (long long)z.stride, pieces, (int)per_row, (int)z.cols, tokens, (const float*)lse,
                           (const float*)entropy, (const float*)dlogprob, (const float*)dentropy, (T*)dz.data, (long long)dz.stride);
         }
