@@ -719,14 +719,16 @@ __global__ void __launch_bounds__(kThreads) logprobs_backward_rows_kernel(const 
     }
 }
 
-// Everything else streams: a CTA takes kBatch packets a thread of one row, all loaded before the first is worked on, and p is
-// exp2 of t = (z - lse) log2 e.  With dentropy:  dz = -p (g + w (log p + H)) = -p (a + b t),  a = g + w H, b = w / log2 e.
-template <typename T, bool ENTROPY>
+// Everything else streams: a CTA (a warp, where rows are short) takes kBatch packets a thread of one row, all loaded before the first
+// is worked on, and p is exp2 of t = (z - lse) log2 e.  With dentropy:  dz = -p (g + w (log p + H)) = -p (a + b t),  a = g + w H, b = w / log2 e.
+template <typename T, int WR, bool ENTROPY>
 __global__ void __launch_bounds__(kThreads) logprobs_backward_kernel(const T* logits, long long ld, long long pieces, int per_row, int vocab,
                                                                      const int* __restrict__ tokens, const float* __restrict__ lse,
                                                                      const float* __restrict__ entropy, const float* __restrict__ dlogprob,
                                                                      const float* __restrict__ dentropy, T* dlogits, long long ldd) {
-    constexpr int N = Packet<T>::N;
+    constexpr int N = Packet<T>::N, TEAM = 32 * WR, TEAMS = kThreads / TEAM;
+    const int me = threadIdx.x % TEAM;
+    const long long mine = (long long)blockIdx.x * TEAMS + threadIdx.x / TEAM, step = (long long)gridDim.x * TEAMS;
     dependent_prologue();
     // what a row's entries need, read a piece ahead: the packets can be asked for at once
     struct Row { int t; float g, l, w, h; };
@@ -740,32 +742,33 @@ __global__ void __launch_bounds__(kThreads) logprobs_backward_kernel(const T* lo
         v.h = ENTROPY ? entropy[r] : 0.0f;
         return v;
     };
-    Row next = row_of(blockIdx.x);
-    for (long long piece = blockIdx.x; piece < pieces; piece += gridDim.x) {
+    Row next = {};
+    if (mine < pieces) next = row_of(mine);
+    for (long long piece = mine; piece < pieces; piece += step) {
         const long long r = piece / per_row;
         const int part = (int)(piece - r * per_row);
         const RowSplit<T> row(logits + r * ld, vocab);
         T* out = dlogits + r * ldd;
         const int t = next.t;
         const float g = t < 0 ? 0.0f : t >= vocab ? nan_of(0.0f) : next.g, l = next.l, w = next.w, h = next.h;
-        if (piece + gridDim.x < pieces) next = row_of(piece + gridDim.x);
+        if (piece + step < pieces) next = row_of(piece + step);
         const bool nothing = (g == 0 && w == 0) || l == -infinity_of(0.0f);
         const float a = -(g + w * h), b = -w * kLn2;
-        const int begin = part * kBatch * kThreads + threadIdx.x;
+        const int begin = part * kBatch * TEAM + me;
         if (nothing) {          // 0 whatever the logits hold: they are not read
 #pragma unroll
             for (int i = 0; i < kBatch; ++i)
-                if (begin + i * kThreads < row.packets) *reinterpret_cast<uint4*>(out + row.first_of(begin + i * kThreads)) = make_uint4(0, 0, 0, 0);
-            if (part == 0 && (int)threadIdx.x < row.head + row.tail) out[row.edge(threadIdx.x)] = Narrow<T>::of(0.0f);
+                if (begin + i * TEAM < row.packets) *reinterpret_cast<uint4*>(out + row.first_of(begin + i * TEAM)) = make_uint4(0, 0, 0, 0);
+            if (part == 0 && me < row.head + row.tail) out[row.edge(me)] = Narrow<T>::of(0.0f);
             continue;
         }
         uint4 q[kBatch];
 #pragma unroll
         for (int i = 0; i < kBatch; ++i)
-            if (begin + i * kThreads < row.packets) q[i] = row.packet(begin + i * kThreads);
+            if (begin + i * TEAM < row.packets) q[i] = row.packet(begin + i * TEAM);
 #pragma unroll
         for (int i = 0; i < kBatch; ++i) {
-            const int p = begin + i * kThreads;
+            const int p = begin + i * TEAM;
             if (p >= row.packets) break;
             Two z[N / 2];
             pairs_of(q[i], z, (const T*)nullptr);
@@ -787,8 +790,8 @@ __global__ void __launch_bounds__(kThreads) logprobs_backward_kernel(const T* lo
             }
             __stcs(reinterpret_cast<uint4*>(out + row.first_of(p)), packet_of(z, (const T*)nullptr));
         }
-        if (part == 0 && (int)threadIdx.x < row.head + row.tail) {
-            const int j = row.edge(threadIdx.x);
+        if (part == 0 && me < row.head + row.tail) {
+            const int j = row.edge(me);
             const float t0 = max_nan((widen(row.z[j]) - l) * kLog2e, kFloor);
             out[j] = Narrow<T>::of(exp2_of(t0) * (t0 * b + a) + (j == t ? g : 0.0f));
         }
@@ -842,9 +845,13 @@ cudaError_t backward(cudaStream_t s, const Rows& z, const int* tokens, const voi
     const bool alike = ((uintptr_t)z.data - (uintptr_t)dz.data) % 16 == 0 && (z.rows < 2 || (z.stride - dz.stride) * z.size % 16 == 0);
     if constexpr (sizeof(T) < 8) {
         if (alike) {
-            const long long packets = z.cols / Packet<T>::N, per_row = std::max<long long>(1, (packets + kBatch * kThreads - 1) / (kBatch * kThreads));
+            const long long packets = z.cols / Packet<T>::N;
+            const bool warp_each = packets <= 32 * kBatch * 4;          // (16384 x 1000 f32: 41 us with a CTA per row)
+            const long long piece = kBatch * (warp_each ? 32 : kThreads), per_row = std::max<long long>(1, (packets + piece - 1) / piece);
             const long long pieces = z.rows * per_row;
-            return launch(dentropy ? logprobs_backward_kernel<T, true> : logprobs_backward_kernel<T, false>, dim3((unsigned)capped(pieces, kSms * 8)),
+            auto kernel = warp_each ? (dentropy ? logprobs_backward_kernel<T, 1, true> : logprobs_backward_kernel<T, 1, false>)
+                                    : (dentropy ? logprobs_backward_kernel<T, kWarps, true> : logprobs_backward_kernel<T, kWarps, false>);
+            return launch(kernel, dim3((unsigned)capped(warp_each ? (pieces + kWarps - 1) / kWarps : pieces, kSms * 8)),
                           kThreads, 0, s, 1, (const T*)z.data, (long long)z.stride, pieces, (int)per_row, (int)z.cols, tokens, (const float*)lse,
                           (const float*)entropy, (const float*)dlogprob, (const float*)dentropy, (T*)dz.data, (long long)dz.stride);
         }
