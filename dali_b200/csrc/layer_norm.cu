@@ -159,6 +159,11 @@ __global__ void __launch_bounds__(kThreads) fold_columns_kernel(const A* __restr
 // are one more for each of the row's first threads.  A CTA's rows are a multiple of W apart, so that every thread holds the same
 // columns of all of them.  (W = 1: matrices whose rows do not even lie alike on the grid.)
 enum Rowfit { FULL, WHOLE, EDGE };          // every thread holds C packets; packets are there or not; EDGE
+__host__ __device__ constexpr int lanes_of(int warps) {          // a lane for each of them: the power of two above
+    int n = 1;
+    while (n < warps) n *= 2;
+    return n;
+}
 template <int W, int C, int WR, Rowfit FIT>
 struct Held {
     uint32_t there;          // bit i: the thread's i-th packet is one of the row's
@@ -174,7 +179,8 @@ struct Held {
             if (t + i * 32 * WR < packets) there |= 1u << i;
         if (FIT == EDGE && t < edges) edge = t < head ? t : t + packets * W;
         mine = of_warp(t >> 5, packets, edges);
-        its = of_warp(t & 31 & (WR - 1), packets, edges);
+        const int w = t % lanes_of(WR);
+        its = w < WR ? of_warp(w, packets, edges) : 0;
     }
     __device__ __forceinline__ int column(int i) const { return first + i * 32 * WR * W; }
     __device__ __forceinline__ bool has(int i) const { return FIT == FULL || (there >> i & 1); }
@@ -281,11 +287,11 @@ struct Vals<1> {
     template <bool GRID, typename P> __device__ __forceinline__ void weights(const P* w) { f = widen(*w); }
 };
 
-// over WR neighbouring lanes
+// over the lanes that stand for WR warps
 template <int WR>
 __device__ __forceinline__ float sum_of(float v) {
 #pragma unroll
-    for (int m = WR / 2; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
+    for (int m = lanes_of(WR) / 2; m > 0; m >>= 1) v += __shfl_xor_sync(0xffffffffu, v, m);
     return v;
 }
 
@@ -295,15 +301,14 @@ __device__ __forceinline__ float quotient(float s, int n, float per_n) {
     return __fmaf_rn(__fmaf_rn(-m, (float)n, s), per_n, m);
 }
 
-// The threads that share a row meet: at most four groups of a CTA, each at a barrier of its own.  (A barrier whose number is
-// computed would count as all sixteen.)
+// The threads that share a row meet: the two groups of a CTA at a barrier each (one whose number is computed would count as all
+// sixteen), more of them at one, and go from row to row together.
+__host__ __device__ constexpr bool meet(int warps, int groups) { return warps > 1 && groups > 2; }
 template <int WR, int GROUPS>
 __device__ __forceinline__ void row_barrier(int group) {
-    if (GROUPS == 1) __syncthreads();
+    if (GROUPS != 2) __syncthreads();
     else if (group == 0) asm volatile("bar.sync 1, %0;" ::"n"(32 * WR) : "memory");
-    else if (group == 1) asm volatile("bar.sync 2, %0;" ::"n"(32 * WR) : "memory");
-    else if (group == 2) asm volatile("bar.sync 3, %0;" ::"n"(32 * WR) : "memory");
-    else asm volatile("bar.sync 4, %0;" ::"n"(32 * WR) : "memory");
+    else asm volatile("bar.sync 2, %0;" ::"n"(32 * WR) : "memory");
 }
 
 template <typename T, typename P, int W, int C, int WR, int GROUPS, int DEPTH, int CTAS, Rowfit FIT>
@@ -311,6 +316,7 @@ __global__ void __launch_bounds__(32 * WR * GROUPS, CTAS) norm_resident_kernel(c
                                                                                const P* __restrict__ beta, T* y, long long ldy,
                                                                                long long rows, int cols, float eps) {
     constexpr int THREADS = 32 * WR * GROUPS;
+    constexpr bool MEET = meet(WR, GROUPS);
     extern __shared__ uint4 ring[];          // [DEPTH][C][THREADS]
     __shared__ float2 sm[2][GROUPS * WR];
     dependent_prologue();
@@ -351,19 +357,21 @@ __global__ void __launch_bounds__(32 * WR * GROUPS, CTAS) norm_resident_kernel(c
         for (int d = 0; d < DEPTH - 1; ++d) fetch(d);
     int stage = 0, turn = 0;
     const float edge_g = gamma && at.has_edge() ? widen(gamma[at.edge]) : 1.0f, edge_b = beta && at.has_edge() ? widen(beta[at.edge]) : 0.0f;
-    float edge_next = at.has_edge() && row < rows ? widen(from[at.edge]) : 0.0f;          // a row ahead
-    for (; row < rows; row += step, from += step * ldx, to += step * ldy) {
+    T edge_next = T();          // a row ahead, and as it was read: widened here, the thread would wait for it
+    if (at.has_edge() && row < rows) edge_next = from[at.edge];
+    for (; row - (MEET ? group : 0) < rows; row += step, from += step * ldx, to += step * ldy) {
+        const bool live = !MEET || row < rows;
         if (W > 1) {
             fetch(stage ? stage - 1 : DEPTH - 1);
             copies_but<DEPTH - 1>();
         }
         Vals<W> v[C];
-        const float edge = edge_next;
-        if (at.has_edge() && row + step < rows) edge_next = widen(from[step * ldx + at.edge]);
+        const float edge = widen(edge_next);
+        if (at.has_edge() && row + step < rows) edge_next = from[step * ldx + at.edge];
         float sum = edge;
 #pragma unroll
         for (int i = 0; i < C; ++i) {
-            if (at.has(i)) v[i].read(W > 1 ? (const T*)(ring + (stage * C + i) * THREADS + threadIdx.x) : from + at.column(i));
+            if (at.has(i) && (W > 1 || live)) v[i].read(W > 1 ? (const T*)(ring + (stage * C + i) * THREADS + threadIdx.x) : from + at.column(i));
             else v[i].all(0);
             sum += v[i].sum();
         }
@@ -387,7 +395,8 @@ __global__ void __launch_bounds__(32 * WR * GROUPS, CTAS) norm_resident_kernel(c
             turn ^= 1;
             if (lane == 0) all[warp] = make_float2(sum, q);
             row_barrier<WR, GROUPS>(group);
-            const float2 o = all[lane % WR];
+            const int other = lane % lanes_of(WR);
+            const float2 o = other < WR ? all[other] : make_float2(0, 0);
             mean = quotient(sum_of<WR>(o.x), cols, per_col);
             const float d = o.x * per_its - mean;
             q = sum_of<WR>(o.y + its * d * d);
@@ -395,7 +404,7 @@ __global__ void __launch_bounds__(32 * WR * GROUPS, CTAS) norm_resident_kernel(c
         const float r = rsqrtf(q * per_col + eps);
 #pragma unroll
         for (int i = 0; i < C; ++i)
-            if (at.has(i)) {
+            if (at.has(i) && live) {
                 v[i].add(-mean);          // (exact for a row that does not vary, where r is largest)
                 v[i].mul(r);
                 if (HOLD) {
@@ -413,7 +422,7 @@ __global__ void __launch_bounds__(32 * WR * GROUPS, CTAS) norm_resident_kernel(c
                 }
                 v[i].write(to + at.column(i));
             }
-        if (at.has_edge()) to[at.edge] = Narrow<T>::of((edge - mean) * r * edge_g + edge_b);
+        if (at.has_edge() && live) to[at.edge] = Narrow<T>::of((edge - mean) * r * edge_g + edge_b);
         stage = stage + 1 == DEPTH ? 0 : stage + 1;
     }
 }
@@ -425,6 +434,7 @@ __global__ void __launch_bounds__(32 * WR * GROUPS, CTAS)
     norm_backward_resident_kernel(const T* dy, long long lddy, const T* x, long long ldx, const P* __restrict__ gamma, T* dx, long long lddx,
                                   long long rows, int cols, float eps, float* __restrict__ partial) {
     constexpr int THREADS = 32 * WR * GROUPS;
+    constexpr bool MEET = meet(WR, GROUPS);
     extern __shared__ uint4 ring[];          // [DEPTH][2][C][THREADS]; in the end [2][cols] sums, where several groups have some to add
     __shared__ float4 sm[2][GROUPS * WR];
     dependent_prologue();
@@ -438,7 +448,11 @@ __global__ void __launch_bounds__(32 * WR * GROUPS, CTAS)
     // Up to 16 values a thread, the row and its weights stay in registers across the exchange; above, they are read again behind it
     // (the row from the ring, the weights from L1), and the sums of the columns have the registers.
     constexpr bool HOLD = C * W <= 16;
-    constexpr int H = HOLD ? C : 1;
+    // 16-bit rows whose threads do not all hold the same stay in their packets between the two passes, half the registers for one
+    // more unpacking (without it 13419 x 5001 spilled: 208 us, now 139; 67108 x 1000 took 98 us, now 93).  Where 8 or more warps
+    // share a row on the grid, nothing spills, and unpacking costs 3%.
+    constexpr bool PACKED = HOLD && W > 1 && sizeof(T) == 2 && (FIT == EDGE || (FIT == WHOLE && WR < 8));
+    constexpr int H = HOLD ? C : 1, R = PACKED ? 1 : H, K = PACKED ? C : 1;
     Vals<W> g[H], dg[C], db[C];
     auto weigh = [&](int i) {
         g[HOLD ? i : 0].all(1);
@@ -472,36 +486,55 @@ __global__ void __launch_bounds__(32 * WR * GROUPS, CTAS)
         for (int d = 0; d < DEPTH - 1; ++d) fetch(d);
     int stage = 0, turn = 0;
     const float edge_g = gamma && at.has_edge() ? widen(gamma[at.edge]) : 1.0f;
-    float edge_dg = 0, edge_db = 0, edge_x_next = 0, edge_dy_next = 0;          // (the next row's: a row ahead)
+    float edge_dg = 0, edge_db = 0;
+    T edge_x_next = T(), edge_dy_next = T();          // a row ahead
     if (at.has_edge() && row < rows) {
-        edge_x_next = widen(from_x[at.edge]);
-        edge_dy_next = widen(from_dy[at.edge]);
+        edge_x_next = from_x[at.edge];
+        edge_dy_next = from_dy[at.edge];
     }
-    for (; row < rows; row += step, from_x += step * ldx, from_dy += step * lddy, to_dx += step * lddx) {
+    for (; row - (MEET ? group : 0) < rows; row += step, from_x += step * ldx, from_dy += step * lddy, to_dx += step * lddx) {
+        const bool live = !MEET || row < rows;
         if (W > 1) {
             fetch(stage ? stage - 1 : DEPTH - 1);
             copies_but<DEPTH - 1>();
         }
-        Vals<W> v[H], u[H];
-        float edge_x = edge_x_next, edge_dy = edge_dy_next;
+        Vals<W> v[R], u[R];
+        uint4 px[K], pdy[K];
+        float edge_x = widen(edge_x_next), edge_dy = widen(edge_dy_next);
         if (at.has_edge() && row + step < rows) {
-            edge_x_next = widen(from_x[step * ldx + at.edge]);
-            edge_dy_next = widen(from_dy[step * lddy + at.edge]);
+            edge_x_next = from_x[step * ldx + at.edge];
+            edge_dy_next = from_dy[step * lddy + at.edge];
         }
         float sum = edge_x;
         auto read_x = [&](int i) {
-            v[HOLD ? i : 0].read(W > 1 ? (const T*)slot(stage, 0, i) : from_x + at.column(i));
+            if constexpr (PACKED) v[0].read((const T*)&px[i]);
+            else v[HOLD ? i : 0].read(W > 1 ? (const T*)slot(stage, 0, i) : from_x + at.column(i));
         };
         auto read_dy = [&](int i) {
-            u[HOLD ? i : 0].read(W > 1 ? (const T*)slot(stage, 1, i) : from_dy + at.column(i));
+            if constexpr (PACKED) u[0].read((const T*)&pdy[i]);
+            else u[HOLD ? i : 0].read(W > 1 ? (const T*)slot(stage, 1, i) : from_dy + at.column(i));
+        };
+        auto again = [&] {          // the values are taken out of their packets anew
+            if constexpr (PACKED) {
+#pragma unroll
+                for (int i = 0; i < C; ++i) {
+                    asm volatile("" : "+r"(px[i].x), "+r"(px[i].y), "+r"(px[i].z), "+r"(px[i].w));
+                    asm volatile("" : "+r"(pdy[i].x), "+r"(pdy[i].y), "+r"(pdy[i].z), "+r"(pdy[i].w));
+                }
+            }
         };
 #pragma unroll
         for (int i = 0; i < C; ++i)
-            if (at.has(i)) {
+            if (at.has(i) && (W > 1 || live)) {
+                if constexpr (PACKED) {
+                    px[i] = *slot(stage, 0, i);
+                    pdy[i] = *slot(stage, 1, i);
+                }
                 read_x(i);
-                if (HOLD) read_dy(i);
-                sum += v[HOLD ? i : 0].sum();
+                if (HOLD && !PACKED) read_dy(i);
+                sum += v[R > 1 ? i : 0].sum();
             }
+        again();
         sum = warp_sum(sum);
         const float mean_w = sum * per_mine;
         Vals<W> sq, sa, sc;
@@ -511,15 +544,15 @@ __global__ void __launch_bounds__(32 * WR * GROUPS, CTAS)
 #pragma unroll
         for (int i = 0; i < C; ++i)
             if (at.has(i)) {
-                const int k = HOLD ? i : 0;
-                if (!HOLD) {
+                const int k = R > 1 ? i : 0, w = HOLD ? i : 0;
+                if ((!HOLD || PACKED) && (W > 1 || live)) {
                     read_x(i);
                     read_dy(i);
-                    weigh(i);
                 }
+                if (!HOLD) weigh(i);
                 Vals<W> d = v[k], ae = u[k];
                 d.add(-mean_w);
-                ae.mul(g[k]);
+                ae.mul(g[w]);
                 sq.fma(d, d, sq);
                 sa.add(ae);
                 sc.fma(ae, d, sc);
@@ -540,33 +573,35 @@ __global__ void __launch_bounds__(32 * WR * GROUPS, CTAS)
             turn ^= 1;
             if (lane == 0) all[warp] = make_float4(sum, q, a, c);
             row_barrier<WR, GROUPS>(group);
-            const float4 o = all[lane % WR];
+            const int other = lane % lanes_of(WR);
+            const float4 o = other < WR ? all[other] : make_float4(0, 0, 0, 0);
             mean = quotient(sum_of<WR>(o.x), cols, per_col);
             const float d = o.x * per_its - mean;      // (a warp without elements has o.x = o.z = 0)
             q = sum_of<WR>(o.y + its * d * d);
             a = sum_of<WR>(o.z);
             c = sum_of<WR>(o.w + o.z * d);
         }
+        again();
         const float r = rsqrtf(q * per_col + eps);
         const float c1 = -r * (a * per_col), c2 = -r * r * (r * (c * per_col));
 #pragma unroll
         for (int i = 0; i < C; ++i)
-            if (at.has(i)) {
-                const int k = HOLD ? i : 0;
-                if (!HOLD) {
+            if (at.has(i) && live) {
+                const int k = R > 1 ? i : 0, w = HOLD ? i : 0;
+                if (!HOLD || PACKED) {
                     read_x(i);
                     read_dy(i);
-                    weigh(i);
                 }
+                if (!HOLD) weigh(i);
                 v[k].add(-mean);          // h / r
                 db[i].add(u[k]);
                 u[k].mul(r);
                 dg[i].fma(u[k], v[k], dg[i]);
-                u[k].fma(u[k], g[k], c1);
+                u[k].fma(u[k], g[w], c1);
                 u[k].fma(v[k], c2, u[k]);
                 if (dx) u[k].write(to_dx + at.column(i));
             }
-        if (at.has_edge()) {
+        if (at.has_edge() && live) {
             edge_x -= mean;
             edge_db += edge_dy;
             edge_dy *= r;
@@ -614,8 +649,11 @@ Layout forward_layout(int size, int64_t cols) {
     Layout l = {size == 2 ? 2 : 4, 1};
     if (packets <= 32ll * l.packets / 2) l.packets /= 2;
     else if (size == 2 && packets > 32 * 32 * 2) l.packets = 4;
-    while (l.warps <= 32 && 32ll * l.packets * l.warps < packets) l.warps *= 2;
-    if (l.warps > 32) l.warps = 0;
+    for (int warps : {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 32}) {
+        l.warps = warps;
+        if (32ll * l.packets * warps >= packets) return l;
+    }
+    l.warps = 0;
     return l;
 }
 // Backward: 16 values a thread for bf16 rows (16384 x 4096: 82 us; 8 values 103), 8 for f32 rows (65536 x 1024: 127 us; 16 values 144);
@@ -624,7 +662,10 @@ Layout backward_layout(int size, int64_t cols) {
     const int64_t packets = (cols + 16 / size - 1) / (16 / size);
     Layout l = {size == 2 && packets <= 32 ? 1 : 2, 1};
     const int most = size == 2 ? 16 : 32;
-    while (l.warps <= most && 32ll * l.packets * l.warps < packets) l.warps *= 2;
+    for (int warps : {1, 2, 3, 4, 5, 8, 16, 32, 64}) {
+        l.warps = warps;
+        if (32ll * l.packets * warps >= packets) break;
+    }
     if (l.warps > most) l = {size == 2 ? 4 : 8, 32ll * 16 * (size == 2 ? 4 : 8) < packets ? 0 : 16};
     return l;
 }
@@ -644,10 +685,12 @@ long long column_slices(long long rows, long long cols) {
     return capped((kSms * 8 + tiles - 1) / tiles, std::max<long long>(1, rows / 4));
 }
 
-// A CTA that holds 16 values a thread in 256 threads takes half of an SM's registers.
+// 16 values a thread take 128 registers: 16 warps an SM, or 15.
+constexpr int backward_groups_of(int warps) { return warps == 3 ? 5 : groups_of(warps); }
+constexpr int backward_resident_ctas(int threads) { return threads > 256 ? 1 : threads > 160 ? 2 : 3; }
 long long backward_ctas(const Layout& l, int64_t rows) {
-    const int groups = groups_of(l.warps);
-    return capped_alike((rows + groups - 1) / groups, kSms * (l.warps > 8 ? 1 : 2));
+    const int groups = backward_groups_of(l.warps);
+    return capped_alike((rows + groups - 1) / groups, kSms * backward_resident_ctas(32 * groups * l.warps));
 }
 
 struct BackwardSpace { size_t stats, partial, total; long long slices; };
@@ -683,19 +726,21 @@ constexpr int kDepth = 3;
 template <typename T, typename P, int C, int WR>
 cudaError_t forward_resident(cudaStream_t s, const Rows& x, const void* gamma, const void* beta, const Rows& y, double eps) {
     constexpr int N = Packet<T>::N, GROUPS = groups_of(WR), THREADS = 32 * WR * GROUPS;
-    constexpr int CTAS = THREADS == 256 ? (C * N > 16 ? 2 : C * N > 8 ? 3 : 4) : THREADS == 512 ? (C * N > 8 ? 1 : 2) : 1;
+    constexpr int CTAS = std::max(1, (C * N > 16 ? 512 : C * N > 8 ? 768 : 1024) / THREADS);          // (80 registers a thread hold 16 values)
+    // (16 values and a thread's edge want some registers more; with two CTAs in place of three: 67041 x 1001 bf16 86 -> 59 us)
+    constexpr int EC = C * N > 8 && THREADS <= 256 ? 512 / THREADS : CTAS;
     const bool vec = alike(x, y);
     const bool whole = vec && on_grid(x) && x.cols % N == 0 && on_grid(gamma) && on_grid(beta), full = whole && x.cols == (int64_t)32 * WR * C * N;
     auto kernel = full    ? norm_resident_kernel<T, P, N, C, WR, GROUPS, kDepth, CTAS, FULL>
                   : whole ? norm_resident_kernel<T, P, N, C, WR, GROUPS, kDepth, CTAS, WHOLE>
-                  : vec   ? norm_resident_kernel<T, P, N, C, WR, GROUPS, kDepth, CTAS, EDGE>
+                  : vec   ? norm_resident_kernel<T, P, N, C, WR, GROUPS, kDepth, EC, EDGE>
                           : norm_resident_kernel<T, P, 1, C * N, WR, GROUPS, kDepth, CTAS, WHOLE>;
     const size_t smem = vec ? (size_t)kDepth * C * THREADS * 16 : 0;
     static std::atomic<unsigned long long> allowed[3];
     const cudaError_t e = allow_shared(kernel, smem, &allowed[full ? 0 : whole ? 1 : 2]);
     if (e != cudaSuccess) return e;
     const long long ctas = (x.rows + GROUPS - 1) / GROUPS;
-    return launch(kernel, dim3((unsigned)capped_alike(ctas, kSms * (vec ? CTAS : 32))), THREADS, smem, s, 1,
+    return launch(kernel, dim3((unsigned)capped_alike(ctas, kSms * (vec ? whole ? CTAS : EC : 32))), THREADS, smem, s, 1,
                   (const T*)x.data, (long long)x.stride, (const P*)gamma, (const P*)beta, (T*)y.data, (long long)y.stride,
                   (long long)x.rows, (int)x.cols, (float)eps);
 }
@@ -704,7 +749,12 @@ cudaError_t forward_resident(cudaStream_t s, int warps, const Rows& x, const voi
     switch (warps) {
         case 1: return forward_resident<T, P, C, 1>(s, x, gamma, beta, y, eps);
         case 2: return forward_resident<T, P, C, 2>(s, x, gamma, beta, y, eps);
+        case 3: return forward_resident<T, P, C, 3>(s, x, gamma, beta, y, eps);
         case 4: return forward_resident<T, P, C, 4>(s, x, gamma, beta, y, eps);
+        case 5: return forward_resident<T, P, C, 5>(s, x, gamma, beta, y, eps);
+        case 6: return forward_resident<T, P, C, 6>(s, x, gamma, beta, y, eps);
+        case 10: return forward_resident<T, P, C, 10>(s, x, gamma, beta, y, eps);
+        case 12: return forward_resident<T, P, C, 12>(s, x, gamma, beta, y, eps);
         case 8: return forward_resident<T, P, C, 8>(s, x, gamma, beta, y, eps);
         case 16: return forward_resident<T, P, C, 16>(s, x, gamma, beta, y, eps);
         default: return forward_resident<T, P, C, 32>(s, x, gamma, beta, y, eps);
@@ -735,8 +785,8 @@ cudaError_t fold_columns(cudaStream_t s, const A* partial, long long slices, lon
 template <typename T, typename P, int C, int WR>
 cudaError_t backward_resident(cudaStream_t s, const BackwardSpace& b, const Rows& dy, const Rows& x, const void* gamma, const Rows& dx,
                               void* dgamma, void* dbeta, double eps, void* space) {
-    constexpr int N = Packet<T>::N, GROUPS = groups_of(WR), THREADS = 32 * WR * GROUPS;
-    constexpr int CTAS = THREADS == 256 ? 2 : 1;
+    constexpr int N = Packet<T>::N, GROUPS = backward_groups_of(WR), THREADS = 32 * WR * GROUPS;
+    constexpr int CTAS = backward_resident_ctas(THREADS);
     constexpr int DEPTH = C * N > 16 ? (sizeof(T) == 2 ? 2 : 1) : kDepth;          // (what fits an SM's shared memory)
     const bool vec = alike(x, dy) && (!dx.data || alike(x, dx));
     const bool whole = vec && on_grid(x) && x.cols % N == 0 && on_grid(gamma), full = whole && x.cols == (int64_t)32 * WR * C * N;
@@ -758,7 +808,9 @@ cudaError_t backward_resident_of(int warps, R... rest) {
     switch (warps) {
         case 1: return backward_resident<T, P, C, 1>(rest...);
         case 2: return backward_resident<T, P, C, 2>(rest...);
+        case 3: return backward_resident<T, P, C, 3>(rest...);
         case 4: return backward_resident<T, P, C, 4>(rest...);
+        case 5: return backward_resident<T, P, C, 5>(rest...);
         case 8: return backward_resident<T, P, C, 8>(rest...);
         case 16: return backward_resident<T, P, C, 16>(rest...);
         default:
