@@ -122,6 +122,33 @@ def test_long_rows_and_many_rows(lib, shape, types):
     test_backward(lib, shape, types)
 
 
+@pytest.mark.parametrize("types", TYPES[:3])
+@pytest.mark.parametrize("cols", [300, 301, 640, 703, 760, 761, 1152, 1201, 1275, 1500, 1505, 2400, 2497, 2990, 5000, 5003, 6000, 6007])
+def test_rows_by_any_number_of_warps(lib, cols, types):
+    """Widths that a number of warps which is no power of two covers, on the grid and off it; rows that end inside a CTA's groups,
+    and matrices that lie unlike one another."""
+    dt, wt = types
+    rng = np.random.default_rng(cols)
+    for rows, shift in ((1, 0), (13, 0), (13, 1), (1501, 0)):
+        _, x = matrix(rng, rows, cols, dt)
+        _, dy = matrix(rng, rows, cols, dt, offset=shift, spread=1.0)
+        gamma = torch.from_numpy(1 + 0.3 * rng.standard_normal(cols)).cuda().to(TORCH[wt])
+        beta = torch.from_numpy(0.3 * rng.standard_normal(cols)).cuda().to(TORCH[wt])
+        bo, out = matrix(rng, rows, cols, dt, offset=shift)
+        bo.fill_(77.0)
+        lib.layer_norm(dt, wt, rows, cols, x, gamma, beta, out, eps=EPS)
+        agree(out, *Formula(x, gamma, beta, dt).y(), dt)
+        bx, dx = matrix(rng, rows, cols, dt)
+        bx.fill_(77.0)
+        dg, db = (torch.empty(cols, device="cuda", dtype=TORCH[wt]) for _ in range(2))
+        lib.layer_norm_backward(dt, wt, rows, cols, dy, x, gamma, dx, dg, db, eps=EPS)
+        want = Formula(x, gamma, None, dt).grads(dy, rows)
+        agree(dx, *want[0], dt)
+        agree(dg, *want[1], wt)
+        agree(db, *want[2], wt)
+        assert (bo[:shift] == 77.0).all() and (bo[shift + rows * cols:] == 77.0).all() and (bx[rows * cols:] == 77.0).all()
+
+
 @pytest.mark.parametrize("types", TYPES)
 @pytest.mark.parametrize("rows,cols", [(6, 1000), (150, 1024), (5, 513), (700, 96), (3, 33000)])
 def test_strides_offsets_and_writing_over_an_input(lib, rows, cols, types):
