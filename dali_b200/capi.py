@@ -3,6 +3,7 @@
 Nothing here computes: every call goes into libdali_b200.so, and loading fails
 loudly when the library has not been built.
 """
+import array
 import ctypes
 import os
 
@@ -321,41 +322,46 @@ class Library:
             device, stream, dtype, rows, vocab, a(logits), vocab if row_stride is None else row_stride, a(tokens), a(lse), a(entropy),
             a(dlogprob), a(dentropy), a(dlogits), vocab if dlogits_row_stride is None else dlogits_row_stride))
 
+    # Lists of host numbers go through array.array: a quarter of what filling a ctypes array from its elements takes, which for the
+    # gradients of a small model is more than the kernels.  (The caller holds what a list's address is taken of.)
     @staticmethod
     def _addresses(tensors):
-        return (_P * len(tensors))(*[x if x is None or type(x) is int else x.data_ptr() for x in tensors])
+        try:
+            return array.array("q", [x.data_ptr() for x in tensors])
+        except AttributeError:
+            return array.array("q", [x.data_ptr() if hasattr(x, "data_ptr") else int(x or 0) for x in tensors])
 
-    def _tensor_list(self, dtypes, numel, tensors):
+    def _tensor_list(self, dtypes, numel, tensors, outs=None):
         n = len(tensors)
         if len(dtypes) != n or len(numel) != n:
             raise ValueError("dtypes, numel and tensors must have one entry per tensor")
-        return n, (_I * n)(*dtypes), (_L * n)(*numel), self._addresses(tensors)
+        if outs is not None and len(outs) != n:
+            raise ValueError("outs must have one entry per tensor")
+        lists = [array.array("i", dtypes), array.array("q", numel), self._addresses(tensors)]
+        if outs is not None:
+            lists.append(self._addresses(outs))
+        return lists, (n, *[x.buffer_info()[0] for x in lists])
 
     def sum_squares(self, dtypes, numel, tensors, out, workspace=None, device=0, stream=None):
         """*out (fp64) = sum of the squares of all elements of a list of contiguous tensors."""
-        self.check(self.c.dalib200_sum_squares(device, stream, *self._tensor_list(dtypes, numel, tensors), self._address(out),
-                                               *self._workspace(workspace)))
+        lists, args = self._tensor_list(dtypes, numel, tensors)
+        self.check(self.c.dalib200_sum_squares(device, stream, *args, self._address(out), *self._workspace(workspace)))
 
     def global_norm(self, dtypes, numel, tensors, norm, norm_dtype=F32, workspace=None, device=0, stream=None):
         """*norm = the norm of a list of contiguous tensors taken as one vector."""
-        self.check(self.c.dalib200_global_norm(device, stream, *self._tensor_list(dtypes, numel, tensors), norm_dtype,
-                                               self._address(norm), *self._workspace(workspace)))
-
-    def _outs(self, n, outs):
-        if len(outs) != n:
-            raise ValueError("outs must have one entry per tensor")
-        return self._addresses(outs)
+        lists, args = self._tensor_list(dtypes, numel, tensors)
+        self.check(self.c.dalib200_global_norm(device, stream, *args, norm_dtype, self._address(norm), *self._workspace(workspace)))
 
     def scale_to_norm(self, dtypes, numel, tensors, outs, sum_squares, max_norm, device=0, stream=None):
         """outs[i] = tensors[i] * min(1, max_norm / sqrt(*sum_squares))."""
-        args = self._tensor_list(dtypes, numel, tensors)
-        self.check(self.c.dalib200_scale_to_norm(device, stream, *args, self._outs(args[0], outs), self._address(sum_squares), max_norm))
+        lists, args = self._tensor_list(dtypes, numel, tensors, outs)
+        self.check(self.c.dalib200_scale_to_norm(device, stream, *args, self._address(sum_squares), max_norm))
 
     def clip_by_global_norm(self, dtypes, numel, tensors, outs, max_norm, norm, norm_dtype=F32, workspace=None, device=0, stream=None):
         """outs[i] = tensors[i] * min(1, max_norm / n), n the norm of all of them, which is left in *norm."""
-        args = self._tensor_list(dtypes, numel, tensors)
-        self.check(self.c.dalib200_clip_by_global_norm(device, stream, *args, self._outs(args[0], outs), max_norm, norm_dtype,
-                                                       self._address(norm), *self._workspace(workspace)))
+        lists, args = self._tensor_list(dtypes, numel, tensors, outs)
+        self.check(self.c.dalib200_clip_by_global_norm(device, stream, *args, max_norm, norm_dtype, self._address(norm),
+                                                       *self._workspace(workspace)))
 
     def global_norm_workspace(self, n_tensors):
         return self.c.dalib200_global_norm_workspace(n_tensors)
