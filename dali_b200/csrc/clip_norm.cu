@@ -9,6 +9,11 @@
 // The tensors of a list are cut into chunks; the kernels take the list by value (pointers, sizes and first chunk of each, up
 // to kList tensors a launch).  Every CTA of the summing kernel writes one partial sum, and whoever needs the total folds the
 // partials in their order, so results do not depend on scheduling and nothing waits.
+//
+// Bound by memory: the squares of 4e8 bf16 elements 126 us (a copy's rate over the bytes read: 97%; 181 us before a thread's next
+// packets were under way while it worked on some), clipped 398 us.  The gradients are read twice, what is left of them in L2 apart:
+// whether they have to be scaled is known when all of them have been read.  Short lists (six tensors
+// of 1e6 elements together, 17 us a call) are bound by the host: the list, its checks and the launches.
 #include <algorithm>
 #include <cmath>
 #include <vector>
@@ -197,6 +202,8 @@ std::string gather_list(int n, const int* dtypes, const int64_t* numel, const vo
     if (n < 0) return "negative number of tensors";
     if (n > 0 && (!dtypes || !numel || !in)) return "the list's dtypes, numel or pointers are null";
     std::vector<Range> ranges;
+    if (out) ranges.reserve(2 * (size_t)n);
+    t->lists.reserve(((size_t)n + kList - 1) / kList);
     List* l = nullptr;
     // chunks of a size that gives every CTA several, and of one packet a thread at least
     int64_t all = 0;
@@ -204,13 +211,13 @@ std::string gather_list(int n, const int* dtypes, const int64_t* numel, const vo
     int chunk = kMinChunk;
     while (chunk < kMaxChunk && (int64_t)chunk * kMaxCtas * 4 < all) chunk *= 2;
     for (int i = 0; i < n; ++i) {
-        const std::string who = "tensor " + std::to_string(i);
-        if (!floating(dtypes[i])) return who + ": dtype must be f32, f64 or bf16";
-        if (numel[i] < 0 || numel[i] > (int64_t(1) << 48)) return who + ": number of elements out of range";
+        const auto who = [i] { return "tensor " + std::to_string(i); };
+        if (!floating(dtypes[i])) return who() + ": dtype must be f32, f64 or bf16";
+        if (numel[i] < 0 || numel[i] > (int64_t(1) << 48)) return who() + ": number of elements out of range";
         if (numel[i] == 0) continue;
         const int size = size_of(dtypes[i]);
-        if (!in[i] || (out && !out[i])) return who + " is a null pointer";
-        if ((uintptr_t)in[i] % size || (out && (uintptr_t)out[i] % size)) return who + " is not aligned to its elements";
+        if (!in[i] || (out && !out[i])) return who() + " is a null pointer";
+        if ((uintptr_t)in[i] % size || (out && (uintptr_t)out[i] % size)) return who() + " is not aligned to its elements";
         if (out) {
             const uintptr_t a = (uintptr_t)in[i], b = (uintptr_t)out[i], bytes = (uintptr_t)numel[i] * size;
             if (a != b) ranges.push_back({a, a + bytes, i, false});
@@ -271,6 +278,18 @@ std::string wrong_norm(const void* norm, int norm_dtype, int n, const int64_t* n
     return "";
 }
 
+std::string wrong_workspace(const void* workspace, const void* norm, int norm_dtype, int n, const int64_t* numel, const int* dtypes,
+                            const void* const* in, void* const* out) {
+    const size_t need = partial_bytes(n);
+    if (meets(workspace, need, norm, size_of(norm_dtype))) return "the workspace overlaps the result";
+    for (int i = 0; i < n; ++i) {
+        const size_t bytes = (size_t)numel[i] * size_of(dtypes[i]);
+        if (meets(workspace, need, in[i], bytes) || (out && meets(workspace, need, out[i], bytes)))
+            return "the workspace overlaps tensor " + std::to_string(i);
+    }
+    return "";
+}
+
 }  // namespace
 }  // namespace dalib
 
@@ -284,6 +303,7 @@ static int total_of(const char* name, int device, void* stream, int n, const int
         Tensors t;
         std::string w = gather_list(n, dtypes, numel, in, nullptr, &t);
         if (w.empty()) w = wrong_norm(out, out_dtype, n, numel, dtypes, in, nullptr);
+        if (w.empty()) w = wrong_workspace(workspace, out, out_dtype, n, numel, dtypes, in, nullptr);
         if (!w.empty()) return refuse(std::string(name) + ": " + w);
         OnDevice on(device);
         if (on.status != DALIB200_OK) return on.status;
@@ -332,6 +352,7 @@ extern "C" int dalib200_clip_by_global_norm(int device, void* stream, int n_tens
         Tensors t;
         std::string w = n_tensors > 0 && !outs ? "outs is a null pointer" : gather_list(n_tensors, dtypes, numel, tensors, outs, &t);
         if (w.empty()) w = wrong_norm(norm, norm_dtype, n_tensors, numel, dtypes, tensors, outs);
+        if (w.empty()) w = wrong_workspace(workspace, norm, norm_dtype, n_tensors, numel, dtypes, tensors, outs);
         if (!w.empty()) return refuse("dalib200_clip_by_global_norm: " + w);
         OnDevice on(device);
         if (on.status != DALIB200_OK) return on.status;

@@ -145,12 +145,19 @@ __global__ void __launch_bounds__(kThreads) fold_columns_kernel(const A* __restr
 }
 
 // ---------------------------------------------------------------------------------------------- rows held in registers
-// f32 and bf16 rows that fit: some warps share a row, a thread keeps packets of it.  Statistics need one exchange between the warps: each warp takes its own mean first (shuffles), then
+// f32 and bf16 rows that fit: some warps share a row, a thread keeps packets of it, so that every row is read once and written once.
+// Statistics need one exchange between the warps: each warp takes its own mean first (shuffles), then
 //   Q = sum (x - mean_w)^2,  A = sum a,  C = sum a (x - mean_w)
 // about it, and the warps' values are moved to the row's mean as they are added:
 //   sum (x - mean)^2 = sum_w Q_w + n_w (mean_w - mean)^2,   sum a (x - mean) = sum_w C_w + A_w (mean_w - mean).
 // No squares of values far from zero are subtracted from one another, and the backward pass needs no more exchanges with
 // recomputed statistics than it would with saved ones.
+//
+// What bounds them, beside the 6570 GB/s of a copy.  Forward: memory (16384 x 4096 bf16 with f32 weights 45 us, 91%; 4096 x 8192 f32
+// 43 us, 95%), and for rows that end off the 16-byte grid the elements at their edges (33537 x 2001 bf16 58 us, 70%).  Backward, f32:
+// memory (32768 x 1024 67 us, 91%).  Backward, bf16: issue slots (51% taken) and the latency of a row's sums behind one another, with the
+// 16 warps that 128 registers a thread leave an SM (16384 x 4096 85 us, 72%; 13104 x 5121 136 us, 45%).  There, more values a
+// thread, rows read again from shared memory in place of registers (136 us) and fewer shuffles for the sums gained nothing.
 
 // A thread holds C packets of W elements of a row, the row's WR warps side by side.  Packets come through a ring of DEPTH rows in
 // shared memory that every thread fills and reads for itself (cp.async; no thread waits for another one's copies), so that the
@@ -642,8 +649,10 @@ __global__ void __launch_bounds__(32 * WR * GROUPS, CTAS)
 struct Layout { int packets, warps; };
 constexpr int groups_of(int warps) { return warps < 8 ? 8 / warps : 1; }
 
+// The warps are as few as hold the row: a lane without packets costs as much as one with them (13107 x 5120 bf16: 48 us with 10
+// warps, 74 with 16).
 // Forward, measured at 2^26 elements: 16 values a thread (16384 x 4096 bf16: 43 us; 8 values 53, 32 values 58), 8 where a warp can hold
-// the row with them (65536 x 256 f32: 23 us; two warps 23 to 29), 32 for rows that 8 warps cannot hold with 16.
+// the row with them (65536 x 256 f32: 23 us; two warps 23 to 29), 32 for bf16 rows that 32 warps cannot hold with 16.
 Layout forward_layout(int size, int64_t cols) {
     const int64_t packets = (cols + 16 / size - 1) / (16 / size);
     Layout l = {size == 2 ? 2 : 4, 1};
@@ -657,7 +666,8 @@ Layout forward_layout(int size, int64_t cols) {
     return l;
 }
 // Backward: 16 values a thread for bf16 rows (16384 x 4096: 82 us; 8 values 103), 8 for f32 rows (65536 x 1024: 127 us; 16 values 144);
-// 32 for rows that 16 warps cannot hold with these.
+// 32 for rows that 16 warps cannot hold with these.  No 6, 10 or 12 warps: what they save on lanes, the SM loses with 12 or 10 warps
+// in place of 16.
 Layout backward_layout(int size, int64_t cols) {
     const int64_t packets = (cols + 16 / size - 1) / (16 / size);
     Layout l = {size == 2 && packets <= 32 ? 1 : 2, 1};
@@ -956,6 +966,12 @@ extern "C" int dalib200_layer_norm_backward(int device, void* stream, int dtype,
             for (void* w : {dgamma, dbeta})
                 if (meets(w, w_bytes, m->data, (size_t)(m->end() - m->begin())))
                     return refuse("dalib200_layer_norm_backward: a weight's gradient overlaps dy or x");
+        for (const Rows* m : {&mdy, &mx, &mdx})
+            if (m->data && meets(workspace, need.total, m->data, (size_t)(m->end() - m->begin())))
+                return refuse(std::string("dalib200_layer_norm_backward: the workspace overlaps ") + m->name);
+        for (const void* w : {gamma, (const void*)dgamma, (const void*)dbeta})
+            if (meets(workspace, need.total, w, w_bytes))
+                return refuse("dalib200_layer_norm_backward: the workspace overlaps a weight or its gradient");
         OnDevice on(device);
         if (on.status != DALIB200_OK) return on.status;
         std::unique_lock<std::mutex> together(launch_mutex(), std::defer_lock);

@@ -13,7 +13,7 @@ std::mutex& launch_mutex() {
 }
 
 namespace {
-struct Space { void* data = nullptr; size_t bytes = 0; };
+struct Space { void* data = nullptr; size_t bytes = 0; unsigned long long stream_id = 0; };
 // apart from the exchange space of generated kernels: those are queued without the launch mutex
 std::map<std::pair<int, void*>, Space>& spaces() {
     static auto* m = new std::map<std::pair<int, void*>, Space>();
@@ -35,8 +35,11 @@ int workspace_for(int device, void* stream, size_t need, void* given, size_t giv
         cudaGetLastError();
         return refuse("a call that is captured into a graph needs a workspace of its own");
     }
+    // a stream made where a destroyed one lay has another id, and kernels of the destroyed one may still be running
+    unsigned long long id = 0;
+    if (cudaStreamGetId((cudaStream_t)stream, &id) != cudaSuccess) cudaGetLastError();
     Space& s = spaces()[std::make_pair(device, stream)];
-    if (s.bytes < need) {
+    if (s.bytes < need || s.stream_id != id) {
         // (kernels in flight may still use the old block: cudaFree waits for the device)
         const size_t bytes = std::max<size_t>(need, 4u << 20);
         void* fresh = nullptr;
@@ -49,6 +52,7 @@ int workspace_for(int device, void* stream, size_t need, void* given, size_t giv
         if (s.data) cudaFree(s.data);
         s.data = fresh;
         s.bytes = bytes;
+        s.stream_id = id;
     }
     *out = s.data;
     return DALIB200_OK;

@@ -2,6 +2,8 @@
 
 The squares are summed in fp64: the norm is off by half a step of its type (plus n 2^-53).  The factor is rounded to fp32 and the
 product to the tensor's type: 2^-24 twice and half a step."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -212,6 +214,23 @@ def test_streams_and_graphs(lib):
         with pytest.raises(DaliB200Error, match="workspace"):
             lib.global_norm(d, n, t, norms[0], stream=torch.cuda.current_stream().cuda_stream)
     del graphs, g
+
+
+def test_a_stream_that_lies_where_another_one_lay(lib):
+    """Kernels of a destroyed stream may still be using what it was given: a new stream gets space of its own, whatever its address."""
+    rt = torch.cuda.cudart()
+    big, small = torch.full((1 << 26,), 0.5, device="cuda"), torch.full((1 << 10,), 2.0, device="cuda")
+    torch.cuda.synchronize()
+    norms = torch.zeros(8, 2, device="cuda")
+    torch.cuda.synchronize()
+    for i in range(8):
+        for j, t in enumerate((big, small)):
+            handle = ctypes.c_void_p()
+            assert int(rt.cudaStreamCreate(ctypes.addressof(handle))) == 0
+            lib.global_norm([F32], [t.numel()], [t], norms[i, j:], stream=handle.value)
+            assert int(rt.cudaStreamDestroy(handle.value)) == 0
+    torch.cuda.synchronize()
+    assert (norms[:, 0] == 4096.0).all() and (norms[:, 1] == 64.0).all()
 
 
 def test_more_than_2_to_the_31_elements(lib):

@@ -26,6 +26,22 @@ def accepted(f, *args, **kw):
     assert "device index out of range" in str(e.value), str(e.value)
 
 
+class Space:
+    """A workspace at an address that nobody reads."""
+
+    def __init__(self, at, size):
+        self.at, self.size = at, size
+
+    def data_ptr(self):
+        return self.at
+
+    def numel(self):
+        return self.size
+
+    def element_size(self):
+        return 1
+
+
 def test_layer_norm(lib):
     f = lib.layer_norm
     accepted(f, F32, F32, 4, 100, A, B, C, D)
@@ -65,6 +81,10 @@ def test_layer_norm_backward(lib):
     refused("overlaps dy or x", f, F32, F32, 4, 100, A, B, None, C, A + 800, None)
     refused("dx overlaps a weight", f, F32, F32, 4, 100, A, B, None, C, C + 400, None)
     refused("dy is a null pointer", f, F32, F32, 4, 100, None, B, None, C, D, None)
+    need = lib.layer_norm_backward_workspace(F32, 4, 100)
+    for at, name in ((A + 1584, "dy"), (B, "x"), (C - need + 16, "dx"), (D + 384, "a weight"), (D + 784, "a weight")):
+        refused("the workspace overlaps " + name, f, F32, F32, 4, 100, A, B, None, C, D, D + 400, workspace=Space(at, need))
+    accepted(f, F32, F32, 4, 100, A, B, None, C, D, D + 400, workspace=Space(A + 1600, need))
     assert lib.layer_norm_backward_workspace(F32, 0, 100) == 0
     assert lib.layer_norm_backward_workspace(F32, 4, 100) > 0
 
@@ -127,6 +147,11 @@ def test_lists(lib):
         refused("max_norm", lib.clip_by_global_norm, *ok, [A, B], bad, C)
         refused("max_norm", lib.scale_to_norm, *ok, [A, B], C, bad)
     # the same tensor twice, and tensors that share elements, where one of them is written
+    need = lib.global_norm_workspace(1)
+    refused("the workspace overlaps tensor 0", lib.global_norm, [F32], [100], [A], C, workspace=Space(A + 384, need))
+    refused("the workspace overlaps the result", lib.global_norm, [F32], [100], [A], C, workspace=Space(C, need))
+    refused("the workspace overlaps tensor 0", lib.clip_by_global_norm, [F32], [100], [A], [B], 1.0, C, workspace=Space(B - need + 16, need))
+    accepted(lib.clip_by_global_norm, [F32], [100], [A], [B], 1.0, C, workspace=Space(D, need))
     refused("overlaps another", lib.clip_by_global_norm, [F32, F32], [100, 100], [A, A], [A, A], 1.0, C)
     refused("overlaps another", lib.clip_by_global_norm, [F32, F32], [100, 100], [A, A], [A, D], 1.0, C)
     refused("overlaps another", lib.clip_by_global_norm, [F32, F32], [100, 100], [A, B], [D, D + 396], 1.0, C)
