@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(kThreads) fold_columns_kernel(const A* __restr
 //
 // What bounds them, beside the 6570 GB/s of a copy.  Forward: memory (16384 x 4096 bf16 with f32 weights 45 us, 91%; 4096 x 8192 f32
 // 43 us, 95%), and for rows that end off the 16-byte grid the elements at their edges (33537 x 2001 bf16 58 us, 70%).  Backward, f32:
-// memory (32768 x 1024 67 us, 91%).  Backward, bf16: issue slots (51% taken) and the latency of a row's sums behind one another, with the
+// memory (32768 x 1024 67 us, 91%).  Backward, bf16: issue slots (45% taken) and the latency of a row's sums behind one another, with the
 // 16 warps that 128 registers a thread leave an SM (16384 x 4096 85 us, 72%; 13104 x 5121 136 us, 45%).  There, more values a
 // thread, rows read again from shared memory in place of registers (136 us) and fewer shuffles for the sums gained nothing.
 

@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_rows_kernel(const T* __rest
 // pool be too small (all of a few threads' entries larger than every other's), entries are sorted 32 at a time and merged.
 //
 // What bounds it, beside the 6570 GB/s of a copy: memory for f32 rows (4096 x 32768 85 us, 96%); for bf16 rows, with twice the entries a
-// byte, the exponential of each (that unit is busy 60% of the time, 62% of the issue slots are taken) and, in a long run, the clock that
+// byte, the exponential of each (that unit is busy 65% of the time, 70% of the issue slots are taken) and, in a long run, the clock that
 // is left under the power limit (8192 x 65536 177 us alone, 92%; 211 us one call after the other, at 1.7 GHz).  20 alternatives
 // of each of those rows add 80 us, and 5 of 1000 x 50001 f32 13 us: the row's threads wait for one another several times while no row
 // is read.
