@@ -22,6 +22,8 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxTop = DALIB200_MAX_TOP;
+// Index of an entry where a loop steps past the row's end: vocab + kThreads may exceed 2^31 - 1, 2^32 - 1 it does not.
+typedef uint32_t Place;
 
 __device__ __forceinline__ float exp_of(float x) { return expf(x); }
 __device__ __forceinline__ double exp_of(double x) { return exp(x); }
@@ -131,7 +133,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_rows_kernel(const T* __rest
         const T* z = logits + row * ld;
         Running<A> r;
         r.clear();
-        for (int j = threadIdx.x; j < vocab; j += kThreads) r.take(widen(z[j]));
+        for (Place j = threadIdx.x; j < (Place)vocab; j += kThreads) r.take(widen(z[j]));
 #pragma unroll
         for (int m = 16; m > 0; m >>= 1) {
             Running<A> o;
@@ -156,8 +158,8 @@ __global__ void __launch_bounds__(kThreads) logprobs_rows_kernel(const T* __rest
         Ranked<A> last;
         for (int k = 0; k < top; ++k) {
             Ranked<A> b = {0, 0xffffffffu};
-            for (int j = threadIdx.x; j < vocab; j += kThreads) {
-                const Ranked<A> c = {ordered(widen(z[j])), (uint32_t)j};
+            for (Place j = threadIdx.x; j < (Place)vocab; j += kThreads) {
+                const Ranked<A> c = {ordered(widen(z[j])), j};
                 if ((k == 0 || last.before(c)) && c.before(b)) b = c;
             }
 #pragma unroll
@@ -713,13 +715,13 @@ __global__ void __launch_bounds__(kThreads) logprobs_backward_rows_kernel(const 
         const A w = dentropy ? dentropy[row] : (A)0, h = dentropy ? entropy[row] : (A)0, l = lse[row];
         if (t >= vocab) g = nan_of(A());
         const bool nothing = (g == 0 && w == 0) || l == -infinity_of(A());
-        for (int j = threadIdx.x; j < vocab; j += kThreads) {
+        for (Place j = threadIdx.x; j < (Place)vocab; j += kThreads) {
             A d = 0;
             if (!nothing) {
                 const A lp = max_nan((A)widen(z[j]) - l, floor_of_difference<A>());
                 const A p = exp_of(lp);
                 d = -p * (g + w * (lp + h));
-                if (j == t) d += g;
+                if ((int)j == t) d += g;
             }
             out[j] = Narrow<T>::of(d);
         }

@@ -425,3 +425,24 @@ def test_offsets_past_32_bits(lib):
     z.copy_(torch.from_numpy(np.random.default_rng(0).standard_normal((3, 1000))).cuda())
     tokens = torch.tensor([3, 4, 999], dtype=torch.int32, device="cuda")
     check_forward(lib, BF16, z, tokens, 3, stride)
+
+
+def test_the_largest_vocabulary(lib):
+    """2^31 - 1 entries a row, where a step past the row's end no longer fits an int: the kernels that go entry by entry (the
+    gradient of rows that lie unlike one another, f64 rows) end with the row and leave what lies in front of it and behind it."""
+    vocab = (1 << 31) - 1
+    token, lse = torch.tensor([vocab - 1], dtype=torch.int32, device="cuda"), torch.zeros(1, device="cuda")
+    z = torch.zeros(vocab, device="cuda", dtype=torch.bfloat16)
+    buf = torch.full((vocab + 18,), 5.0, device="cuda", dtype=torch.bfloat16)
+    dz = buf[9:9 + vocab]
+    assert (z.data_ptr() - dz.data_ptr()) % 16
+    lib.token_logprobs_backward(BF16, 1, vocab, z, token, lse, None, torch.zeros(1, device="cuda"), None, dz)
+    assert (buf[:9] == 5.0).all() and (buf[9 + vocab:] == 5.0).all()
+    assert not dz.view(torch.int16).any()
+    del z, buf, dz
+    z = torch.full((vocab,), -INF, device="cuda", dtype=torch.float64)
+    z[-1] = 2.0
+    z[5] = 1.0
+    logprob, entropy, lse, tl, tt = forward(lib, F64, z[None], token, 1)
+    want = 2.0 + np.log1p(np.exp(-1.0))
+    assert abs(lse.item() - want) < 1e-14 and abs(logprob.item() - (2.0 - want)) < 1e-14 and tt.item() == vocab - 1
