@@ -48,6 +48,16 @@ size_t copy_out(const std::string& s, char* buffer, size_t capacity) {
 }
 
 Array optional(dali_array_t h) { return h ? h->a : Array(); }
+const Array& required(dali_array_t h, const char* op, const char* name) {
+    DALI_ASSERT(h, std::string(op) + " needs " + name);
+    return h->a;
+}
+std::vector<Array> required(const dali_array_t* arrays, int n, const char* op) {
+    DALI_ASSERT(n >= 0 && (n == 0 || arrays), std::string(op) + " needs a list of arrays");
+    std::vector<Array> v;
+    for (int i = 0; i < n; ++i) v.push_back(required(arrays[i], op, ("array " + std::to_string(i)).c_str()));
+    return v;
+}
 
 dali_array_t wrap(const Array& a) {
     dali_array_s* h = new dali_array_s();
@@ -293,13 +303,17 @@ int dali_op_softmax(dali_array_t logits, int axis, dali_array_t* out) {
     return guard([&]() { *out = wrap(op::softmax(logits->a, axis)); });
 }
 int dali_op_layer_norm(dali_array_t x, dali_array_t gamma, dali_array_t beta, double eps, dali_array_t* out) {
-    return guard([&]() { *out = wrap(op::layer_norm(x->a, optional(gamma), optional(beta), eps)); });
+    return guard([&]() {
+        const Array y = op::layer_norm(required(x, "layer_norm", "x"), optional(gamma), optional(beta), eps);
+        if (out) *out = wrap(y);
+    });
 }
 int dali_op_layer_norm_backward(dali_array_t dy, dali_array_t x, dali_array_t gamma, double eps, dali_array_t* dx, dali_array_t* dgamma,
                                 dali_array_t* dbeta) {
     return guard([&]() {
         Array a, b, c;
-        std::tie(a, b, c) = op::layer_norm_backward(dy->a, x->a, optional(gamma), eps);
+        const char* op = "layer_norm_backward";
+        std::tie(a, b, c) = op::layer_norm_backward(required(dy, op, "dy"), required(x, op, "x"), optional(gamma), eps);
         if (dx) *dx = wrap(a);
         if (dgamma) *dgamma = wrap(b);
         if (dbeta) *dbeta = wrap(c);
@@ -310,7 +324,7 @@ int dali_op_token_logprobs(dali_array_t logits, dali_array_t tokens, int top, da
     return guard([&]() {
         DALI_ASSERT(!logprob || tokens, "token_logprobs: logprob needs tokens");
         DALI_ASSERT((!top_logprobs && !top_tokens) || top > 0, "token_logprobs: no alternatives without top > 0");
-        op::TokenLogprobs r = op::token_logprobs(logits->a, optional(tokens), top);
+        op::TokenLogprobs r = op::token_logprobs(required(logits, "token_logprobs", "logits"), optional(tokens), top);
         if (logprob) *logprob = wrap(r.logprob);
         if (entropy) *entropy = wrap(r.entropy);
         if (lse) *lse = wrap(r.lse);
@@ -321,24 +335,24 @@ int dali_op_token_logprobs(dali_array_t logits, dali_array_t tokens, int top, da
 int dali_op_token_logprobs_backward(dali_array_t logits, dali_array_t tokens, dali_array_t lse, dali_array_t entropy,
                                     dali_array_t dlogprob, dali_array_t dentropy, dali_array_t* out) {
     return guard([&]() {
-        *out = wrap(op::token_logprobs_backward(logits->a, optional(tokens), lse->a, optional(entropy), optional(dlogprob),
-                                                optional(dentropy)));
+        const char* op = "token_logprobs_backward";
+        const Array dz = op::token_logprobs_backward(required(logits, op, "logits"), optional(tokens), required(lse, op, "lse"),
+                                                     optional(entropy), optional(dlogprob), optional(dentropy));
+        if (out) *out = wrap(dz);
     });
 }
 int dali_op_global_norm(const dali_array_t* arrays, int n, dali_array_t* out) {
     return guard([&]() {
-        std::vector<Array> v;
-        for (int i = 0; i < n; ++i) v.push_back(arrays[i]->a);
-        *out = wrap(op::global_norm(v));
+        const Array norm = op::global_norm(required(arrays, n, "global_norm"));
+        if (out) *out = wrap(norm);
     });
 }
 int dali_op_clip_by_global_norm(const dali_array_t* arrays, int n, double max_norm, dali_array_t* clipped, dali_array_t* norm) {
     return guard([&]() {
-        std::vector<Array> v, c;
+        std::vector<Array> c;
         Array total;
-        for (int i = 0; i < n; ++i) v.push_back(arrays[i]->a);
-        std::tie(c, total) = op::clip_by_global_norm(v, max_norm);
-        for (int i = 0; i < n; ++i) clipped[i] = wrap(c[i]);
+        std::tie(c, total) = op::clip_by_global_norm(required(arrays, n, "clip_by_global_norm"), max_norm);
+        for (int i = 0; clipped && i < n; ++i) clipped[i] = wrap(c[i]);
         if (norm) *norm = wrap(total);
     });
 }

@@ -99,7 +99,7 @@ int dali_random_set_seed(int seed);
 int dali_op_softmax(dali_array_t logits, int axis, dali_array_t* out);
 /* operators of a token model (not in the reference; the C++ functions of the same names in dali/array/op.h, the entry points
  * behind them in dali_b200.h).  NULL handles: gamma, beta, tokens, and one of the pairs tokens + dlogprob and entropy + dentropy may
- * be left out; NULL results are not wanted. */
+ * be left out, any other is refused; NULL results are not wanted. */
 int dali_op_layer_norm(dali_array_t x, dali_array_t gamma, dali_array_t beta, double eps, dali_array_t* out);
 int dali_op_layer_norm_backward(dali_array_t dy, dali_array_t x, dali_array_t gamma, double eps, dali_array_t* dx, dali_array_t* dgamma,
                                 dali_array_t* dbeta);

@@ -1,5 +1,6 @@
 """The operators of a token model in the Array / op:: front end, without a GPU: shapes, types, refusals, laziness (dry run), and
 what a shard of the rows ends in."""
+import ctypes
 import os
 import sys
 
@@ -182,3 +183,43 @@ def test_shards_of_rows(tmp_path):
         assert said[3].startswith("1:allreduce sum 1")
         assert said[4].startswith("1:allreduce sum 1 f64") and said[5] == "0:-"
         assert said[6:] == ["True", "True", "True"]
+
+
+@pytest.mark.parametrize("text,call", [
+    ("layer_norm needs x", lambda: op.layer_norm(None)),
+    ("layer_norm_backward needs dy", lambda: op.layer_norm_backward(None, f32(3, 5))),
+    ("layer_norm_backward needs x", lambda: op.layer_norm_backward(f32(3, 5), None)),
+    ("token_logprobs needs logits", lambda: op.token_logprobs(None)),
+    ("token_logprobs_backward needs lse", lambda: op.token_logprobs_backward(f32(3, 5), i32(3), None, None, f32(3))),
+    ("token_logprobs_backward needs logits", lambda: op.token_logprobs_backward(None, i32(3), f32(3), None, f32(3))),
+])
+def test_arguments_that_may_not_be_left_out(text, call):
+    with pytest.raises(DaliB200Error) as e:
+        call()
+    assert text in str(e.value), str(e.value)
+
+
+def test_null_handles_and_results_in_c():
+    lib = dali_b200.load_library()
+    c, error = lib.c, lib.last_error
+    handle, eps, one = ctypes.c_void_p, ctypes.c_double(1e-5), ctypes.c_double(1.0)
+    x, y = f32(3, 5), f32(4)
+    two = (handle * 2)(x._h, y._h)
+    # refused: a list with a hole, no list, a negative number of arrays
+    assert c.dali_op_global_norm((handle * 2)(x._h, None), 2, ctypes.byref(handle())) != 0 and "global_norm needs array 1" in error()
+    assert c.dali_op_global_norm(None, 2, ctypes.byref(handle())) != 0 and "global_norm needs a list" in error()
+    assert c.dali_op_clip_by_global_norm(two, -1, one, two, None) != 0 and "clip_by_global_norm needs a list" in error()
+    # not wanted: no result, or some of them
+    assert c.dali_op_layer_norm(x._h, None, None, eps, None) == 0
+    assert c.dali_op_layer_norm_backward(x._h, x._h, None, eps, None, None, None) == 0
+    assert c.dali_op_token_logprobs(x._h, None, 0, None, None, None, None, None) == 0
+    assert c.dali_op_token_logprobs_backward(x._h, i32(3)._h, f32(3)._h, None, f32(3)._h, None, None) == 0
+    assert c.dali_op_global_norm(two, 2, None) == 0
+    assert c.dali_op_clip_by_global_norm(two, 2, one, None, None) == 0
+    norm = handle()
+    assert c.dali_op_clip_by_global_norm(two, 2, one, None, ctypes.byref(norm)) == 0
+    assert Array(_handle=norm).shape == ()
+    clipped = (handle * 2)()
+    assert c.dali_op_clip_by_global_norm(two, 2, one, clipped, None) == 0
+    assert [Array(_handle=handle(h)).shape for h in clipped] == [(3, 5), (4,)]
+    assert c.dali_op_global_norm(None, 0, ctypes.byref(norm)) == 0 and Array(_handle=norm).shape == ()
