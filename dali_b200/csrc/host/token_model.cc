@@ -32,12 +32,11 @@ std::vector<Array> KernelCall::lazy_results(const std::shared_ptr<KernelCall>& c
 
 Array KernelCall::take(int index) {
     if (computed_.empty() || computed_[index].is_stateless()) {
-        bool sharded = false;
+        const bool all = collective();
         std::vector<Array> in, out;
         Array on;
         for (const Array& a : inputs_) {
             if (a.is_stateless()) { in.push_back(Array()); continue; }
-            sharded = sharded || a.shard().sharded();
             if (on.is_stateless()) on = a;
             Array b = a;
             if (!b.is_buffer()) b.eval(false);
@@ -46,7 +45,7 @@ Array KernelCall::take(int index) {
         const memory::Device device = on.is_stateless() ? memory::default_preferred_device : on.preferred_device();
         for (int i = 0; i < (int)results_.size(); ++i) {
             const Result& r = results_[i];
-            if (i != index && !sharded && nodes_[i].expired()) { out.push_back(Array()); continue; }
+            if (i != index && !all && nodes_[i].expired()) { out.push_back(Array()); continue; }
             Array a(r.shape, r.dtype, device);
             a.expression()->shard_ = r.shard;
             out.push_back(a);
@@ -156,6 +155,7 @@ struct LayerNormBackwardCall : public KernelCall {
     DType weights_;
     bool combine_ = false;
     std::string name() const override { return "layer_norm_backward"; }
+    bool collective() const override { return combine_; }
     void run(const memory::Device& device, const std::vector<Array>& in, const std::vector<Array>& out) override {
         if (combine_)
             for (int i = 1; i < 3; ++i) note_collective("allreduce sum " + std::to_string(out[i].numel()) + " (gradient of a weight of sharded rows)");
@@ -251,6 +251,11 @@ struct ListCall : public KernelCall {
     bool clip_;
     double max_norm_ = 0;
     std::string name() const override { return clip_ ? "clip_by_global_norm" : "global_norm"; }
+    bool collective() const override {
+        for (const Array& a : inputs_)
+            if (a.shard().sharded()) return true;
+        return false;
+    }
     // inputs: the list; results: (clipped arrays,) norm
     void run(const memory::Device& device, const std::vector<Array>& in, const std::vector<Array>& out) override {
         std::vector<int> dtypes[2];
@@ -258,8 +263,7 @@ struct ListCall : public KernelCall {
         std::vector<const void*> from[2];
         std::vector<void*> to;
         std::vector<Array> keep;
-        bool sharded = false;
-        for (const Array& a : in) sharded = sharded || a.shard().sharded();
+        const bool sharded = collective();
         if (sharded) note_collective("allreduce sum 1 f64 (squares of sharded arrays)");
         if (lazy::dry_run()) return;
         const int dev = lazy::device_index(device);

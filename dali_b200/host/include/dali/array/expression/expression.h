@@ -90,8 +90,8 @@ struct Scan : public Expression {
 
 // An operator with a hand-written kernel of its own and one or more results (layer_norm_backward's three gradients): the
 // first result that is asked for runs it, the others find theirs computed.  Like a Scan it is never fused with what
-// consumes it.  Results nobody holds a node of any more are not computed (of whole arrays; of shards they are, so that all
-// ranks take the same collective steps).
+// consumes it.  Results nobody holds a node of any more are not computed, unless the call takes collective steps: those
+// all ranks take alike, whatever each of them still holds.
 struct KernelResult;
 struct KernelCall {
     struct Result { std::string name; std::vector<int> shape; DType dtype; Shard shard; };
@@ -99,6 +99,8 @@ struct KernelCall {
     std::vector<Result> results_;
     virtual ~KernelCall() {}
     virtual std::string name() const = 0;
+    // does a run combine something over the ranks?
+    virtual bool collective() const { return false; }
     // inputs as evaluated buffers; outputs[i] is stateless where the result is not wanted
     virtual void run(const memory::Device& device, const std::vector<Array>& inputs, const std::vector<Array>& outputs) = 0;
     // the lazy Arrays of `call`'s results, one for each

@@ -234,3 +234,33 @@ def test_lists_whose_results_are_not_all_wanted():
     np.testing.assert_array_equal(clipped[3].numpy(), a[1].reshape(10, 100).T)
     assert op.global_norm([]).item() == 0 and op.clip_by_global_norm([], 1.0)[1].item() == 0
     assert norm.dtype == DTYPE_DOUBLE
+
+
+def test_shards_of_rows_without_tokens(lib):
+    """Nothing of token_logprobs crosses ranks: what a shard's rows give is what those rows give alone, with and without
+    tokens, whichever of the results are held."""
+    rng = np.random.default_rng(8)
+    z = rng.standard_normal((5, 33)).astype(np.float32)
+    t = rng.integers(0, 33, 5).astype(np.int32)
+    want = [a.numpy() for a in op.token_logprobs(Array(z), Array(t), top=3)]
+
+    def nothing(*args):
+        raise AssertionError("no collective step is due")
+
+    lib.comm_init_host(2, 0, nothing, nothing)
+    try:
+        shard = lambda a: Array(a).set_shard(0, 0, 10)                 # noqa: E731
+        lp, h, lse, tl, tt = op.token_logprobs(shard(z))
+        assert lp is None and tl is None and tt is None
+        np.testing.assert_array_equal(lse.numpy(), want[2])
+        np.testing.assert_array_equal(h.numpy(), want[1])
+        for tokens in (None, shard(t)):
+            got = op.token_logprobs(shard(z), tokens, top=3)
+            for g, w in zip(got, want):
+                assert (g is None) == (tokens is None and w is want[0])
+                if g is not None:
+                    np.testing.assert_array_equal(g.numpy(), w)
+        _, _, _, _, tt = op.token_logprobs(shard(z), top=2)
+        np.testing.assert_array_equal(tt.numpy(), want[4][:, :2])
+    finally:
+        lib.comm_destroy()
