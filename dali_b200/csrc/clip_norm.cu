@@ -4,7 +4,8 @@
 //   n = sqrt(sum over the tensors of sum g^2),   out = g max_norm / n  where n > max_norm, else g
 //
 // Squares are summed in fp64: a norm that fp32 can hold does not overflow on the way, and a list of billions of elements
-// loses nothing.  A norm that is not finite scales nothing (the caller sees it in `norm`).
+// loses nothing.  A norm that is not finite as it is reported, in fp32 or in fp64, scales nothing: who steps over a list whose
+// norm reads infinity finds it unchanged, in place too.
 //
 // The tensors of a list are cut into chunks; the kernels take the list by value (pointers, sizes and first chunk of each, up
 // to kList tensors a launch).  Every CTA of the summing kernel writes one partial sum, and whoever needs the total folds the
@@ -168,7 +169,7 @@ __global__ void __launch_bounds__(kThreads, 4) scale_kernel(const __grid_constan
     const double sum = fold_partials(partial, n_partial, sm);
     if (norm && blockIdx.x == 0 && threadIdx.x == 0) write_norm(sum, norm, norm_f64);
     const double n = sqrt(sum);
-    const bool down = n > max_norm && n <= DBL_MAX;
+    const bool down = n > max_norm && (norm_f64 ? n <= DBL_MAX : (float)n <= FLT_MAX);
     const double f = down ? max_norm / n : 1.0;
     // from the end of the list: what has been read last for the sum is still in L2
     for (long long c = l.first[l.n] - 1 - blockIdx.x; c >= 0; c -= gridDim.x) {
@@ -330,8 +331,8 @@ extern "C" int dalib200_global_norm(int device, void* stream, int n_tensors, con
     return total_of("dalib200_global_norm", device, stream, n_tensors, dtypes, numel, tensors, 1, norm, norm_dtype, workspace, workspace_bytes);
 }
 
-extern "C" int dalib200_scale_to_norm(int device, void* stream, int n_tensors, const int* dtypes, const int64_t* numel,
-                                      const void* const* tensors, void* const* outs, const double* sum_squares, double max_norm) {
+int dalib::scale_to_norm(int device, void* stream, int n_tensors, const int* dtypes, const int64_t* numel, const void* const* tensors,
+                         void* const* outs, const double* sum_squares, double max_norm, int norm_dtype) {
     return guarded("dalib200_scale_to_norm", [&]() -> int {
         if (!(max_norm > 0)) return refuse("dalib200_scale_to_norm: max_norm must be a number > 0");
         Tensors t;
@@ -340,8 +341,14 @@ extern "C" int dalib200_scale_to_norm(int device, void* stream, int n_tensors, c
         if (!w.empty()) return refuse("dalib200_scale_to_norm: " + w);
         OnDevice on(device);
         if (on.status != DALIB200_OK) return on.status;
-        return launched("dalib200_scale_to_norm", queue_scale((cudaStream_t)stream, t, sum_squares, 1, max_norm, nullptr, 0));
+        return launched("dalib200_scale_to_norm", queue_scale((cudaStream_t)stream, t, sum_squares, 1, max_norm, nullptr,
+                                                              norm_dtype == DALIB200_F64));
     });
+}
+
+extern "C" int dalib200_scale_to_norm(int device, void* stream, int n_tensors, const int* dtypes, const int64_t* numel,
+                                      const void* const* tensors, void* const* outs, const double* sum_squares, double max_norm) {
+    return scale_to_norm(device, stream, n_tensors, dtypes, numel, tensors, outs, sum_squares, max_norm, DALIB200_F64);
 }
 
 extern "C" int dalib200_clip_by_global_norm(int device, void* stream, int n_tensors, const int* dtypes, const int64_t* numel,

@@ -8,6 +8,7 @@
 #include <cmath>
 
 #include "../../../include/dali_b200.h"
+#include "../op_host.h"
 #include "dali/array/op.h"
 #include "dali/array/expression/expression.h"
 
@@ -324,8 +325,8 @@ struct ListCall : public KernelCall {
         if (clip_) {
             BufferView* b = as<BufferView>(total);
             const double* pt = (const double*)b->memory_->data(device, memory::AM_READONLY) + b->offset_;
-            lazy::check(dalib200_scale_to_norm(dev, nullptr, (int)want_from.size(), want_dtypes.data(), want_numel.data(), want_from.data(),
-                                               to.data(), pt, max_norm_),
+            lazy::check(dalib::scale_to_norm(dev, nullptr, (int)want_from.size(), want_dtypes.data(), want_numel.data(), want_from.data(),
+                                             to.data(), pt, max_norm_, norm.dtype()),
                         "dalib200_scale_to_norm");
         }
     }

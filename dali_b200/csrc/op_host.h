@@ -118,6 +118,10 @@ inline int launched(const char* what, cudaError_t e) {
     return DALIB200_ERR_CUDA;
 }
 
+// dalib200_scale_to_norm for a norm that is reported in norm_dtype: one that is not finite there scales nothing (clip_norm.cu).
+int scale_to_norm(int device, void* stream, int n_tensors, const int* dtypes, const int64_t* numel, const void* const* tensors,
+                  void* const* outs, const double* sum_squares, double max_norm, int norm_dtype);
+
 // No C++ exception leaves a C entry point.
 template <typename F>
 int guarded(const char* what, F f) {

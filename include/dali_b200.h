@@ -314,8 +314,10 @@ int dalib200_token_logprobs_backward(int device, void* stream, int dtype, int64_
  *   scale_to_norm        outs[i] = tensors[i] * min(1, max_norm / n), n = sqrt(*sum_squares): for lists that are spread over
  *                        ranks, whose sums of squares are added (dalib200_allreduce) in between
  *   clip_by_global_norm  all of it: *norm is the norm before scaling
- * outs[i] may be tensors[i]; nothing that is written may overlap anything else of the list.  max_norm > 0.  A norm that is
- * not finite scales nothing: outs[i] = tensors[i], and *norm says so.  Sums are taken in fp64 in a fixed order. */
+ * outs[i] may be tensors[i]; nothing that is written may overlap anything else of the list.  max_norm > 0.  Sums are
+ * taken in fp64 in a fixed order.  A norm that is not finite scales nothing: outs[i] = tensors[i].  What counts is the norm as it is
+ * reported, so an f32 *norm of infinity goes with an unscaled list although fp64 could hold the norm (scale_to_norm, which
+ * reports none, goes by fp64).  Squares of f64 elements beyond 1e154 overflow: such a list's norm is infinity. */
 int dalib200_sum_squares(int device, void* stream, int n_tensors, const int* dtypes, const int64_t* numel,
                          const void* const* tensors, double* sum, void* workspace, size_t workspace_bytes);
 int dalib200_global_norm(int device, void* stream, int n_tensors, const int* dtypes, const int64_t* numel,

@@ -242,3 +242,34 @@ def test_more_than_2_to_the_31_elements(lib):
     assert abs(norm.item() - want) <= want * 2.0 ** -23
     f = torch.tensor([300.0 * np.float32(1.0 / want)], dtype=torch.float32).to(torch.bfloat16).item()
     assert t[-1].item() == f and t[0].item() == torch.tensor([0.5 / want], dtype=torch.float32).to(torch.bfloat16).item()
+
+
+@pytest.mark.parametrize("dt,value", [(F32, 1e38), (BF16, 2.0 ** 126), (F64, 1e38), (F64, 1e150)])
+def test_a_norm_that_its_type_cannot_hold_scales_nothing(lib, dt, value):
+    """100 elements whose norm, 10 times an element, lies beyond fp32's range and inside fp64's: reported in fp32 it is infinity,
+    and nothing is scaled; reported in fp64 it is a number, and the list is scaled to it."""
+    spec = [(90, dt), (10, dt)]
+    t = [torch.full((n,), value, device="cuda", dtype=TORCH[dt]) for n, _ in spec]
+    outs = [torch.full_like(x, 5.0) for x in t]
+    norm = call(lib, spec, t, outs, 2.0)
+    assert norm.item() == float("inf") and all(torch.equal(o, x) for o, x in zip(outs, t))
+    mine = [x.clone() for x in t]
+    assert call(lib, spec, mine, mine, 2.0).item() == float("inf") and all(torch.equal(o, x) for o, x in zip(mine, t))
+    norm = torch.zeros((), device="cuda", dtype=torch.float64)
+    lib.clip_by_global_norm([dt, dt], [90, 10], t, outs, value, norm, norm_dtype=F64)
+    assert abs(norm.item() / (10 * t[0][0].item()) - 1) < 1e-14           # (of the elements as they are stored)
+    for o in outs:            # a tenth of value: the factor and the product rounded to fp32, the result to its type
+        off = (HALF_STEP[dt] + (2 * 2.0 ** -24 if dt != F64 else 2.0 ** -50)) * 1.01
+        assert ((o.double() / (value / 10) - 1).abs() <= off).all()
+
+
+def test_a_norm_next_to_the_end_of_fp32(lib):
+    """The largest norm that rounds to a number of fp32 still scales (to 16: the factor is no subnormal number)."""
+    top = torch.finfo(torch.float32).max
+    t = torch.tensor([top, 0.0], device="cuda")
+    out = torch.empty_like(t)
+    norm = call(lib, [(2, F32)], [t], [out], 16.0)
+    assert norm.item() == top and abs(out[0].item() / 16 - 1) <= 3 * 2.0 ** -24 * 1.01
+    t[1] = top / 2
+    norm = call(lib, [(2, F32)], [t], [out], 16.0)
+    assert norm.item() == float("inf") and torch.equal(out, t)

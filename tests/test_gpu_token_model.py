@@ -264,3 +264,27 @@ def test_shards_of_rows_without_tokens(lib):
         np.testing.assert_array_equal(tt.numpy(), want[4][:, :2])
     finally:
         lib.comm_destroy()
+
+
+def test_a_norm_that_fp32_cannot_hold_scales_nothing(lib):
+    """All of a list, a part of it, and a shard of it (the other rank's rows hold zeros): the same answer."""
+    x, y = np.full((9, 10), 1e38, np.float32), np.full(10, 1e38, np.float32)
+    clipped, norm = op.clip_by_global_norm([Array(x), Array(y)], 1.0)
+    assert norm.item() == np.inf
+    np.testing.assert_array_equal(clipped[0].numpy(), x)
+    np.testing.assert_array_equal(clipped[1].numpy(), y)
+    clipped, norm = op.clip_by_global_norm([Array(x), Array(y)], 1.0)
+    del clipped[0]
+    np.testing.assert_array_equal(clipped[0].numpy(), y)
+    assert norm.item() == np.inf
+    lib.comm_init_host(2, 0, lambda buf, n, dtype, op_code: None, lambda *a: None)
+    try:
+        clipped, norm = op.clip_by_global_norm([Array(x).set_shard(0, 0, 18), Array(y)], 1.0)
+        np.testing.assert_array_equal(clipped[0].numpy(), x)
+        np.testing.assert_array_equal(clipped[1].numpy(), y)
+        assert norm.item() == np.inf
+    finally:
+        lib.comm_destroy()
+    clipped, norm = op.clip_by_global_norm([Array(x.astype(np.float64)), Array(y)], 1e38)
+    assert norm.dtype == DTYPE_DOUBLE and abs(norm.item() / np.float64(np.sqrt(100 * np.float64(np.float32(1e38)) ** 2)) - 1) < 1e-14
+    np.testing.assert_allclose(clipped[0].numpy(), np.full((9, 10), 1e37), rtol=1e-6)
