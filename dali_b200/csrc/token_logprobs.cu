@@ -95,27 +95,24 @@ struct Ranked {
     __device__ __forceinline__ bool before(const Ranked& o) const { return value > o.value || (value == o.value && index < o.index); }
 };
 
-// What a thread of the row's CTA has to say when the statistics are known.
+// A row's normaliser, the largest entry and the logarithm of the sum apart: log p = (z - m) - log s does not depend on what all
+// entries have in common, while m + log s rounded to fp32 (the lse that is written) is off by 2^-24 of it.
 template <typename A>
-__device__ __forceinline__ void finish_row(const Running<A>& all, long long row, A* logprob, A* entropy, A* lse_out, A* lse) {
-    A l, h;
+struct Normaliser {
+    A m, log_s, lse;
+    __device__ __forceinline__ A log_p(A z) const { return lse == -infinity_of(A()) ? lse : (z - m) - log_s; }
+};
+// from the row's sums; u in the units of a difference z - m times `unit`
+template <typename A, typename R>
+__device__ __forceinline__ Normaliser<A> finish_row(const R& all, A unit, A* entropy) {
     if (all.s == 0) {              // nothing but -infinity
-        l = -infinity_of(A());
-        h = 0;
-    } else {
-        const A ls = log_of(all.s);
-        l = all.m + ls;
-        h = ls - all.u / all.s;
+        *entropy = 0;
+        return {all.m, 0, -infinity_of(A())};
     }
-    *lse = l;
-    if (entropy) entropy[row] = h;
-    if (lse_out) lse_out[row] = l;
-    (void)logprob;
+    const A log_s = log_of(all.s);
+    *entropy = log_s - unit * (all.u / all.s);
+    return {all.m, log_s, all.m + log_s};
 }
-
-// log p of an entry
-template <typename A>
-__device__ __forceinline__ A log_p(A z, A lse) { return lse == -infinity_of(A()) ? lse : z - lse; }
 
 // ---------------------------------------------------------------------------------------------- f64 rows
 // A CTA per row, one entry a thread and step; the alternatives one after another, each by another walk over the row.
@@ -147,12 +144,14 @@ __global__ void __launch_bounds__(kThreads) logprobs_rows_kernel(const T* __rest
         __syncthreads();
         Running<A> all = sm[0];
         for (int w = 1; w < kThreads / 32; ++w) all.merge(sm[w]);
-        A lse;
+        A h;
+        const Normaliser<A> norm = finish_row(all, (A)1, &h);
         if (threadIdx.x == 0) {
-            finish_row(all, row, logprob, entropy, lse_out, &lse);
+            if (entropy) entropy[row] = h;
+            if (lse_out) lse_out[row] = norm.lse;
             if (logprob) {
                 const int t = tokens[row];
-                logprob[row] = t < 0 ? (A)0 : t >= vocab ? nan_of(A()) : log_p((A)widen(z[t]), lse);
+                logprob[row] = t < 0 ? (A)0 : t >= vocab ? nan_of(A()) : norm.log_p(widen(z[t]));
             }
         }
         Ranked<A> last;
@@ -177,7 +176,7 @@ __global__ void __launch_bounds__(kThreads) logprobs_rows_kernel(const T* __rest
                 if (best[w].before(last)) last = best[w];
             if (threadIdx.x == 0) {
                 top_tokens[row * top + k] = (int)last.index;
-                top_logprobs[row * top + k] = log_p((A)widen(z[last.index]), lse);
+                top_logprobs[row * top + k] = norm.log_p(widen(z[last.index]));
             }
         }
     }
@@ -664,27 +663,20 @@ __global__ void __launch_bounds__(kThreads, 4) logprobs_kernel(const T* __restri
                 me = sm[lane % kWarps];
                 me.over_lanes<kWarps>();
             }
-            float l, h;
-            if (me.s == 0) {          // nothing but -infinity
-                l = -infinity_of(0.0f);
-                h = 0;
-            } else {
-                const float ls = logf(me.s);
-                l = me.m + ls;
-                h = ls - kLn2 * (me.u / me.s);
-            }
+            float h;
+            const Normaliser<float> norm = finish_row(me, kLn2, &h);
             if (lane == 0) {
                 if (entropy) entropy[r] = h;
-                if (lse_out) lse_out[r] = l;
+                if (lse_out) lse_out[r] = norm.lse;
                 if (logprob) {
                     const int given = tokens[r];
-                    logprob[r] = given < 0 ? 0.0f : given >= vocab ? nan_of(0.0f) : log_p(widen(row.z[given]), l);
+                    logprob[r] = given < 0 ? 0.0f : given >= vocab ? nan_of(0.0f) : norm.log_p(widen(row.z[given]));
                 }
             }
             if (lane < top) {
                 const int index = index_of(lists[0][lane]);
                 top_tokens[r * top + lane] = index;
-                top_logprobs[r * top + lane] = log_p(widen(row.z[index]), l);
+                top_logprobs[r * top + lane] = norm.log_p(widen(row.z[index]));
             }
         }
         if (WR > 1 && cluster > 1) {           // the first CTA has read what the others sent for this row

@@ -446,3 +446,24 @@ def test_the_largest_vocabulary(lib):
     logprob, entropy, lse, tl, tt = forward(lib, F64, z[None], token, 1)
     want = 2.0 + np.log1p(np.exp(-1.0))
     assert abs(lse.item() - want) < 1e-14 and abs(logprob.item() - (2.0 - want)) < 1e-14 and tt.item() == vocab - 1
+
+
+@pytest.mark.parametrize("dt", [F32, BF16, F64])
+@pytest.mark.parametrize("rows,vocab", [(1, 100), (9, 4099), (1300, 1000), (3, 131072), (400, 30001)])
+def test_what_all_entries_have_in_common_costs_no_digits(lib, rows, vocab, dt):
+    """Rows far from 0: log probabilities and entropies are those of the row less its largest entry (which no rounding touches:
+    both are multiples of the same step, a few bits apart), with the error of such a row; lse is off by half a step of itself."""
+    rng = np.random.default_rng(rows + vocab)
+    for common in {F32: (1e3, -1e4, 3e5), BF16: (200.0, -1e3), F64: (1e6, -1e12)}[dt]:
+        z = torch.from_numpy(common + 3.0 * rng.standard_normal((rows, vocab))).cuda().to(TORCH[dt])
+        tokens = torch.from_numpy(rng.integers(-1, vocab, rows).astype(np.int32)).cuda()
+        logprob, entropy, lse, tl, tt = forward(lib, dt, z, tokens, 8)
+        m = z.double().max(1, keepdim=True).values
+        f = Formula(z.double() - m, dt)
+        want = f.logprob(tokens)
+        agree(logprob, want, f.e_logprob(want))
+        agree(entropy, f.entropy, f.e_entropy)
+        agree(lse, m[:, 0] + f.lse, f.e_lse + f.u * (m[:, 0] + f.lse).abs())
+        values, index = f.top(8)
+        assert torch.equal(tt.long(), index)
+        agree(tl, values, f.e_lse[:, None] + f.u * values.abs())
