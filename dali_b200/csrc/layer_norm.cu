@@ -118,7 +118,7 @@ __device__ __forceinline__ void write_gradient(const T* up, const T* in, const P
     });
 }
 
-// Per row: mean, r, mean(a) and r^2 mean(a h / r), 4 values in `stats`, and dx where it is given: where the columns are summed from
+// Per row: mean, r, mean(a) and r^2 mean(a h / r), 4 values in `stats` where the columns are summed behind it, and dx where it is given: where the columns are summed from
 // matrices that dx is written over, dx_kernel writes it behind that.
 template <typename T, typename P, int W>
 __global__ void __launch_bounds__(1024) row_stats_kernel(const T* dy, long long lddy, const T* x, long long ldx, const P* __restrict__ gamma, T* dx,
@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(1024) row_stats_kernel(const T* dy, long long 
         });
         const A r = (A)1 / root(block_sum(q, sm) / (A)cols + (A)eps);
         const A k = r * (r * (block_sum(qa, sm) / (A)cols));
-        if (threadIdx.x == 0) {
+        if (threadIdx.x == 0 && stats) {
             stats[4 * row] = mean;
             stats[4 * row + 1] = r;
             stats[4 * row + 2] = mean_a;
@@ -783,6 +783,7 @@ long long backward_ctas(const Layout& l, int64_t rows) {
     return capped_alike((rows + groups - 1) / groups, kSms * backward_resident_ctas(32 * groups * l.warps));
 }
 
+// What the sums over the rows hand from launch to launch; dx alone comes out of one launch that needs none of it.
 struct BackwardSpace { size_t stats, partial, total; long long slices; };
 BackwardSpace backward_space(int dtype, int64_t rows, int64_t cols) {
     const size_t a = dtype == DALIB200_F64 ? 8 : 4;
@@ -929,7 +930,7 @@ cudaError_t backward(cudaStream_t s, const Rows& dy, const Rows& x, const void* 
             }
         }
     }
-    A* stats = (A*)space;
+    A* stats = (A*)space;          // nullptr: no sums are asked for
     A* partial = (A*)((char*)space + b.stats);
     const bool packets = sizeof(T) < 8 && alike(x, dy) && (!dx.data || alike(x, dx)), sums = dgamma || dbeta;
     const bool late = sums && dx.data && (meets(dx.data, dx.end() - dx.begin(), x.data, x.end() - x.begin()) ||
@@ -1041,7 +1042,7 @@ extern "C" int dalib200_layer_norm_backward(int device, void* stream, int dtype,
             const std::string w = wrong(*m);
             if (!w.empty()) return refuse("dalib200_layer_norm_backward: " + w);
         }
-        const BackwardSpace need = backward_space(dtype, rows, cols);
+        const size_t need = dgamma || dbeta ? backward_space(dtype, rows, cols).total : 0;
         if (dx) {
             if (clash(mdy, mdx)) return refuse("dalib200_layer_norm_backward: dx overlaps dy without being dy");
             if (clash(mx, mdx)) return refuse("dalib200_layer_norm_backward: dx overlaps x without being x");
@@ -1053,18 +1054,22 @@ extern "C" int dalib200_layer_norm_backward(int device, void* stream, int dtype,
             for (void* w : {dgamma, dbeta})
                 if (meets(w, w_bytes, m->data, (size_t)(m->end() - m->begin())))
                     return refuse("dalib200_layer_norm_backward: a weight's gradient overlaps dy or x");
-        for (const Rows* m : {&mdy, &mx, &mdx})
-            if (m->data && meets(workspace, need.total, m->data, (size_t)(m->end() - m->begin())))
-                return refuse(std::string("dalib200_layer_norm_backward: the workspace overlaps ") + m->name);
-        for (const void* w : {gamma, (const void*)dgamma, (const void*)dbeta})
-            if (meets(workspace, need.total, w, w_bytes))
-                return refuse("dalib200_layer_norm_backward: the workspace overlaps a weight or its gradient");
+        if (need) {
+            for (const Rows* m : {&mdy, &mx, &mdx})
+                if (m->data && meets(workspace, need, m->data, (size_t)(m->end() - m->begin())))
+                    return refuse(std::string("dalib200_layer_norm_backward: the workspace overlaps ") + m->name);
+            for (const void* w : {gamma, (const void*)dgamma, (const void*)dbeta})
+                if (meets(workspace, need, w, w_bytes))
+                    return refuse("dalib200_layer_norm_backward: the workspace overlaps a weight or its gradient");
+        }
         OnDevice on(device);
         if (on.status != DALIB200_OK) return on.status;
         std::unique_lock<std::mutex> together(launch_mutex(), std::defer_lock);
-        if (!workspace) together.lock();
         void* space = nullptr;
-        if ((rc = workspace_for(device, stream, need.total, workspace, workspace_bytes, &space)) != DALIB200_OK) return rc;
+        if (need) {
+            if (!workspace) together.lock();
+            if ((rc = workspace_for(device, stream, need, workspace, workspace_bytes, &space)) != DALIB200_OK) return rc;
+        }
         cudaError_t e;
         if (dtype == DALIB200_F32) e = backward<float, float>(s, mdy, mx, gamma, mdx, dgamma, dbeta, eps, space);
         else if (dtype == DALIB200_F64) e = backward<double, double>(s, mdy, mx, gamma, mdx, dgamma, dbeta, eps, space);

@@ -276,7 +276,8 @@ int dalib200_layer_norm(int device, void* stream, int dtype, int param_dtype, in
                         void* out, int64_t out_row_stride);
 /* The gradients of dalib200_layer_norm for the gradient dy of its result: dx [rows, cols], and dgamma, dbeta (`cols` values
  * of param_dtype, overwritten), each of the three optional.  The rows' statistics are computed again from x.  The sums over the rows
- * are taken in a fixed order: the same call gives the same bits. */
+ * are taken in a fixed order: the same call gives the same bits.  The workspace is for those sums: a call without dgamma and dbeta
+ * needs none, on any stream. */
 int dalib200_layer_norm_backward(int device, void* stream, int dtype, int param_dtype, int64_t rows, int64_t cols,
                                  const void* dy, int64_t dy_row_stride, const void* x, int64_t x_row_stride,
                                  const void* gamma, double eps, void* dx, int64_t dx_row_stride, void* dgamma, void* dbeta,

@@ -430,3 +430,37 @@ def test_offsets_past_32_bits(lib):
     out = torch.empty(3, 64, device="cuda", dtype=torch.bfloat16)
     lib.layer_norm(BF16, BF16, 3, 64, x, None, None, out, eps=EPS, x_row_stride=stride)
     agree(out, *Formula(x, None, None, BF16).y(), BF16)
+
+
+@pytest.mark.parametrize("dt", [F32, BF16, F64])
+@pytest.mark.parametrize("cols", [100, 1024, 40000])
+def test_the_gradient_of_the_rows_alone_needs_no_workspace(lib, cols, dt):
+    """In a captured graph, on the per-thread default stream, with a workspace of no size, over an argument: the bits of a call that
+    has all gradients."""
+    rows, rng = 70, np.random.default_rng(cols)
+    x, dy = matrix(rng, rows, cols, dt)[1], matrix(rng, rows, cols, dt, spread=1.0)[1]
+    want, dx, dg, db = (torch.empty(n, cols, device="cuda", dtype=TORCH[dt]) for n in (rows, rows, 1, 1))
+    lib.layer_norm_backward(dt, dt, rows, cols, dy, x, None, want, dg, db, eps=EPS)
+    agree(want, *Formula(x, None, None, dt).grads(dy, rows)[0], dt)
+
+    def right():
+        torch.cuda.synchronize()
+        assert torch.equal(dx, want)
+        dx.zero_()
+        torch.cuda.synchronize()
+
+    alone = (dt, dt, rows, cols, dy, x, None, dx, None, None)
+    right_over = dx.copy_(dy)
+    lib.layer_norm_backward(dt, dt, rows, cols, right_over, x, None, dx, None, None, eps=EPS)
+    right()
+    lib.layer_norm_backward(*alone, eps=EPS, workspace=torch.empty(0, device="cuda"))
+    right()
+    lib.layer_norm_backward(*alone, eps=EPS, stream=2)
+    right()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        lib.layer_norm_backward(*alone, eps=EPS, stream=torch.cuda.current_stream().cuda_stream)
+    for _ in range(3):
+        graph.replay()
+        right()
+    del graph

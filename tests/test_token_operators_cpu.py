@@ -159,3 +159,12 @@ def test_lists(lib):
     accepted(lib.clip_by_global_norm, [F32, F32], [100, 100], [A, A], [B, D], 1.0, C)
     with pytest.raises(ValueError):
         lib.global_norm([F32], [1, 2], [A, B], C, device=-1)
+
+
+def test_a_workspace_that_is_not_needed_is_not_looked_at(lib):
+    """The gradient of the rows alone hands nothing from launch to launch."""
+    f = lib.layer_norm_backward
+    need = lib.layer_norm_backward_workspace(F32, 4, 100)
+    accepted(f, F32, F32, 4, 100, A, B, None, C, None, None, workspace=Space(A, need))
+    refused("the workspace overlaps dy", f, F32, F32, 4, 100, A, B, None, C, D, None, workspace=Space(A, need))
+    refused("the workspace overlaps dy", f, F32, F32, 4, 100, A, B, None, C, None, D, workspace=Space(A, need))
