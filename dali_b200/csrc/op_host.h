@@ -78,7 +78,8 @@ inline bool meets(const void* a, size_t a_bytes, const void* b, size_t b_bytes) 
 }
 
 // The caller's workspace, or space of the library's own for (device, stream), which operators that need more than one launch
-// pass their partial results through (op_host.cc).  The latter is handed to the next call on that stream, so a captured
+// pass their partial results through (op_host.cc).  The latter is handed to the next call on that stream (and kept for it, up
+// to 512 MB a device over all streams), so a captured
 // call, whose graph may be replayed beside anything, has to bring its own, and so has one on the per-thread default stream,
 // whose one handle stands for several streams.  Without a caller's workspace the launches of a call stay together under
 // launch_mutex(), so that two threads that share a stream do not mix their partial results.

@@ -273,3 +273,24 @@ def test_a_norm_next_to_the_end_of_fp32(lib):
     t[1] = top / 2
     norm = call(lib, [(2, F32)], [t], [out], 16.0)
     assert norm.item() == float("inf") and torch.equal(out, t)
+
+
+def test_space_of_many_streams_is_bounded(lib):
+    """Nothing tells the library that a stream is gone: what it keeps for them stays within 512 MB, and a stream whose space went
+    gets another one."""
+    rt = torch.cuda.cudart()
+    handles = [ctypes.c_void_p() for _ in range(200)]
+    assert all(int(rt.cudaStreamCreate(ctypes.addressof(h))) == 0 for h in handles)
+    t = torch.arange(1, 3, device="cuda", dtype=torch.float32)
+    norms = torch.zeros(2, len(handles), device="cuda")
+    lib.global_norm([F32], [2], [t], norms)
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    for again in range(2):
+        for i, h in enumerate(handles):
+            lib.global_norm([F32], [2], [t], norms[again, i:], stream=h.value)
+    torch.cuda.synchronize()
+    taken = free - torch.cuda.mem_get_info()[0]
+    assert all(int(rt.cudaStreamDestroy(h.value)) == 0 for h in handles)
+    assert (norms == torch.tensor(5.0).sqrt().item()).all()
+    assert taken <= (512 + 64) << 20, taken
