@@ -89,7 +89,9 @@ struct Scan : public Expression {
 };
 
 // An operator with a hand-written kernel of its own and one or more results (layer_norm_backward's three gradients): the
-// first result that is asked for runs it, the others find theirs computed.  Like a Scan it is never fused with what
+// first result that is asked for runs it, the others find theirs computed: the results of a call belong to one state of its
+// arguments, the one they had at that moment, also where an argument is changed in place before another result is read (an
+// update of a weight between two of its layer's gradients).  Like a Scan it is never fused with what
 // consumes it.  Results nobody holds a node of any more are not computed, unless the call takes collective steps: those
 // all ranks take alike, whatever each of them still holds.
 struct KernelResult;

@@ -105,7 +105,8 @@ Array gather_from_rows(const Array& source, const Array& indices);
 Array softmax(const Array& logits, int axis = -1);
 Array softmax_temperature(const Array& logits, const Array& temperature, int axis = -1);
 
-// ---- operators of a token model (op/token_model.h; not in the reference).  Lazy, each with a kernel of its own.  Rows run
+// ---- operators of a token model (op/token_model.h; not in the reference).  Lazy, each with a kernel of its own; the results
+// of one call are computed together, from the arguments as they are when the first of them is asked for.  Rows run
 // along the last axis.  Unlike other computations they keep a bf16 type of their rows: a result with the shape of a
 // bf16 argument is bf16 (computed in fp32, rounded once when it is stored).
 // (x - mean) / sqrt(var + eps) * gamma + beta; gamma / beta: vectors of the last axis' length, stateless = left out

@@ -288,3 +288,25 @@ def test_a_norm_that_fp32_cannot_hold_scales_nothing(lib):
     clipped, norm = op.clip_by_global_norm([Array(x.astype(np.float64)), Array(y)], 1e38)
     assert norm.dtype == DTYPE_DOUBLE and abs(norm.item() / np.float64(np.sqrt(100 * np.float64(np.float32(1e38)) ** 2)) - 1) < 1e-14
     np.testing.assert_allclose(clipped[0].numpy(), np.full((9, 10), 1e37), rtol=1e-6)
+
+
+def test_results_of_a_call_belong_to_one_state_of_its_arguments():
+    """The first result asked for runs the call on the arguments of that moment, and its siblings keep to them when an argument
+    changes in place; a call that has not run reads what is there."""
+    rng = np.random.default_rng(9)
+    x, dy, g = (rng.standard_normal(s) for s in ((6, 40), (6, 40), 40))
+    want = [a.numpy() for a in op.layer_norm_backward(Array(dy), Array(x), Array(g))]
+    moved = [a.numpy() for a in op.layer_norm_backward(Array(dy), Array(3 * x), Array(g))]
+    ax, ag = Array(x), Array(g)
+    dx, dg, db = op.layer_norm_backward(Array(dy), ax, ag)
+    np.testing.assert_array_equal(dg.numpy(), want[1])
+    ag -= dg * 0.1                                                    # a solver's step between two gradients of its layer
+    ax *= 3.0
+    np.testing.assert_array_equal(dx.numpy(), want[0])
+    np.testing.assert_array_equal(db.numpy(), want[2])
+    np.testing.assert_allclose(ag.numpy(), g - 0.1 * want[1], rtol=0, atol=1e-15)
+    bx = Array(x)
+    dx, dg, db = op.layer_norm_backward(Array(dy), bx, Array(g))
+    bx *= 3.0
+    for got, w in zip((dg, dx, db), (moved[1], moved[0], moved[2])):
+        np.testing.assert_array_equal(got.numpy(), w)
