@@ -860,10 +860,12 @@ cudaError_t forward(cudaStream_t s, const Rows& x, const void* gamma, const void
     if constexpr (sizeof(T) < 8) {
         const Layout l = forward_layout(sizeof(T), x.cols);
         constexpr int C = sizeof(T) == 2 ? 1 : 2;
-        if (l.warps)
-            return l.packets == C       ? forward_resident<T, P, C, 1>(s, x, gamma, beta, y, eps)
-                   : l.packets == 2 * C ? forward_resident<T, P, 2 * C>(s, l.warps, x, gamma, beta, y, eps)
-                                        : forward_resident<T, P, 4>(s, l.warps, x, gamma, beta, y, eps);
+        if (l.warps) {
+            if (l.packets == C) return forward_resident<T, P, C, 1>(s, x, gamma, beta, y, eps);
+            if constexpr (sizeof(T) == 2)
+                if (l.packets == 4) return forward_resident<T, P, 4, 32>(s, x, gamma, beta, y, eps);          // (above 2048 packets a row)
+            return forward_resident<T, P, 2 * C>(s, l.warps, x, gamma, beta, y, eps);
+        }
     }
     auto kernel = sizeof(T) < 8 && alike(x, y) ? norm_rows_kernel<T, P, packet_width<T>()> : norm_rows_kernel<T, P, 1>;
     return launch(kernel, dim3((unsigned)capped(x.rows, kSms * 64)), row_threads(x.cols), 0, s, 1, (const T*)x.data, (long long)x.stride,
