@@ -464,3 +464,11 @@ def test_the_gradient_of_the_rows_alone_needs_no_workspace(lib, cols, dt):
         graph.replay()
         right()
     del graph
+
+
+@pytest.mark.parametrize("types", TYPES)
+@pytest.mark.parametrize("shape", [(700, 16392), (331, 16401), (620, 20000), (301, 33001)])
+def test_many_rows_wider_than_a_gradient_holds(lib, shape, types):
+    """More rows than CTAs, of widths beyond what the gradient keeps in registers (and for the last ones, the forward pass too)."""
+    test_forward(lib, shape, types)
+    test_backward(lib, shape, types)
