@@ -22,7 +22,8 @@ constexpr int kThreads = 256;
 // f64 rows, and rows that do not fit a CTA's registers.  A CTA walks a row W elements at a time, once for the mean, once for the squared
 // deviations, and once to write it; behind the first walk the row comes from L2.  W is a packet's where the matrices lie alike on the
 // 16-byte grid (the elements in front of it and behind it one by one), else 1.  1 x 17744 f32: 14.3 us with 256 threads and
-// W = 1, 8.6 with 1024 and packets; 4000 x 20000 f32 264 us, 37% of a copy, its gradient 509.
+// W = 1, 8.6 with 1024 and packets; 3000 x 32768 f32 gradient 819 and 576.  Not everywhere: 4000 x 20000 f32 takes 264 us
+// (37% of a copy; its gradient 510) where 256 threads took 244, and the gradient of 3000 x 19999 bf16 388 where they took 373.
 template <int N> struct Width { static constexpr int value = N; };
 template <int W, typename F>
 __device__ __forceinline__ void walk(long long cols, int head, F f) {          // f(Width, column)
@@ -235,9 +236,9 @@ __global__ void __launch_bounds__(kThreads) fold_columns_kernel(const A* __restr
 //
 // What bounds them, beside the 6570 GB/s of a copy.  Forward: memory (16384 x 4096 bf16 with f32 weights 45 us, 91%; 4096 x 8192 f32
 // 43 us, 95%), and for rows that end off the 16-byte grid the elements at their edges (33537 x 2001 bf16 58 us, 70%).  Backward, f32:
-// memory (32768 x 1024 67 us, 91%).  Backward, bf16: issue slots (45% taken) and the latency of a row's sums behind one another, with the
-// 16 warps that 128 registers a thread leave an SM (16384 x 4096 85 us, 72%; 13104 x 5121 136 us, 45%).  There, more values a
-// thread, rows read again from shared memory in place of registers (136 us) and fewer shuffles for the sums gained nothing.
+// memory (32768 x 1024 67 us, 91%).  Backward, bf16: no unit is full (45% of the issue slots taken, DRAM 57%); what is left open is the
+// latency of a row's sums behind one another, with the 16 warps that 128 registers a thread leave an SM (16384 x 4096 83 to 88 us, 70 to
+// 74%; 13104 x 5121 136 us, 45%).  There, more values a thread, rows read again from shared memory in place of registers (136 us) and fewer shuffles for the sums gained nothing.
 
 // A thread holds C packets of W elements of a row, the row's WR warps side by side.  Packets come through a ring of DEPTH rows in
 // shared memory that every thread fills and reads for itself (cp.async; no thread waits for another one's copies), so that the

@@ -292,6 +292,8 @@ size_t dalib200_layer_norm_backward_workspace(int dtype, int64_t rows, int64_t c
  *               nothing else has lse = logprob = -infinity, entropy 0 and alternatives 0, 1, 2, ... of -infinity.  NaN
  *               or +infinity anywhere in a row makes its results NaN; NaN entries rank behind all others among the alternatives.
  *   top         0 .. DALIB200_MAX_TOP, at most vocab
+ * Log probabilities are (z - max) - log sum exp(z - max), as exact in rows far from 0 as in others; lse = max + log sum is rounded once
+ * more, by half a step of itself.  In f32 and bf16 rows exponentials below 2^-126 count as 0.
  * vocab < 2^31. */
 #define DALIB200_MAX_TOP 32
 int dalib200_token_logprobs(int device, void* stream, int dtype, int64_t rows, int64_t vocab,
@@ -301,7 +303,8 @@ int dalib200_token_logprobs(int device, void* stream, int dtype, int64_t rows, i
  * values each, either optional) and the lse and entropy that the forward pass gave:
  *   dlogits[j] = dlogprob ([j == token] - p_j) - dentropy p_j (log p_j + entropy)
  * A row without a token (negative) takes dlogprob as 0; a token >= vocab makes its row NaN.  Rows whose gradients are both
- * 0, and rows of nothing but -infinity, get 0 whatever their logits hold.  entropy is needed with dentropy only, tokens
+ * 0, and rows of nothing but -infinity, get 0 whatever their logits hold.  log p_j is logits[j] - lse with lse as it is given: half a
+ * step of a large lse (2^-24 |lse| in fp32) is a relative error of every p_j, and in f32 and bf16 rows p_j below 2^-126 counts as 0.  entropy is needed with dentropy only, tokens
  * with dlogprob only. */
 int dalib200_token_logprobs_backward(int device, void* stream, int dtype, int64_t rows, int64_t vocab,
                                      const void* logits, int64_t row_stride, const int32_t* tokens,
